@@ -338,6 +338,59 @@ int  dce_debug_latency_trace(dce_ctx* ctx, unsigned long long stamps[16]);
 int  dce_debug_alloc(dce_ctx* ctx, size_t bytes, void** device_ptr);
 int  dce_debug_free(dce_ctx* ctx, void* device_ptr);
 
+/* ---- The matrix products of the FC layers as operators of their own -------------------------------------------------------------------------
+ * Not in the reference, whose FC layers are torch.nn.Linear (src/contact_cnn.py:48-57): the 8-bit form of such a layer, and one layer of many
+ * weight matrices of which every row takes its own (a bank of heads behind one conv stack).  DEVICE pointers only.  These entries hold no state: the
+ * device and the hipStream_t come with the call (NULL: the null stream), launches are asynchronous on it, nothing is allocated, any number of threads
+ * may call at once, and a call may be captured into a graph.  A failure's message is dce_last_error(NULL) of the calling thread. */
+#define DCE_BLOCK       128   /* values along K (and, of weights, rows) that share a scale */
+#define DCE_GROUPS_MAX  1024
+typedef enum dce_type  { DCE_TYPE_F32 = 0, DCE_TYPE_BF16 = 1, DCE_TYPE_E4M3 = 2 } dce_type;   /* E4M3: 8 bits, 4 of them significant, largest 448, no infinity */
+typedef enum dce_scale { DCE_SCALE_E8M0 = 0, DCE_SCALE_F32 = 1 } dce_scale;                  /* E8M0: one byte s, 2^(s - 127), 255 = NaN */
+
+/* x -> e4m3 and a power of two for every block: e = the smallest with max|x| <= 448 * 2^e, held inside [-126, 120]; q = x * 2^-e rounded once, ties to
+ * even.  NaN and infinities become NaN and are left out of the maximum.  block_rows 1: activations, one matrix (batch 1), scale of row i and block t at
+ * scale[t * ld_scale + i].  block_rows 128: weights, `batch` matrices, scale (batch, ceil(rows / 128), ceil(k / 128)) without gaps.  Any k; strides are
+ * in values; x and q may not overlap. */
+typedef struct dce_quantize_desc {
+    const void* x;  int64_t ldx, x_batch;
+    uint8_t*    q;  int64_t ldq, q_batch;
+    void*   scale;  int64_t ld_scale;
+    int64_t batch, rows, k;
+    int32_t x_type /* F32 | BF16 */, scale_type, block_rows, reserved;
+} dce_quantize_desc;
+int  dce_quantize(int device_id, void* hip_stream, const dce_quantize_desc* d);
+
+/* y[j, c] = act( sum over k of a[src(j), k] b[g, c, k] + bias[g, c] ) for the rows offsets[g] <= j < offsets[g + 1]; act = ReLU where relu != 0 (NaN
+ * stays NaN); src(j) = index[j], or j where index is NULL; an index outside [0, a_rows) reads as a row of zeros.  offsets: groups + 1 numbers on the
+ * DEVICE, never falling (NULL: one group of all m rows); they are held inside [0, m]; rows of y that no group covers stay as they were.  Operands bf16,
+ * or e4m3 where a[i, k] stands for a * a_scale[(k / 128) * ld_a_scale + i] and b[g, c, k] for b * b_scale[g * b_scale_group + (c / 128) * ld_b_scale +
+ * k / 128].  fp32 scales may be any finite numbers whose products are normal fp32 numbers or zero.  Sums are fp32; y is rounded once to y_type; e4m3
+ * results take a power of two for every 128 columns of a row, y_scale[(c / 128) * ld_y_scale + j], in scale_type.  Any m, n and k (k = 0: the bias);
+ * strides in values; 16-byte aligned rows run fastest.  y overlaps no operand.  The same call gives the same bits. */
+typedef struct dce_matmul_desc {
+    const void* a; int64_t lda; const void* a_scale; int64_t ld_a_scale;
+    const void* b; int64_t ldb, b_group; const void* b_scale; int64_t ld_b_scale, b_scale_group;
+    const float* bias; int64_t bias_group;                       /* NULL: none */
+    void* y; int64_t ldy; void* y_scale; int64_t ld_y_scale;
+    const int32_t* offsets; const int32_t* index;
+    int64_t a_rows, m, n, k;
+    int32_t groups, in_type /* BF16 | E4M3 */, scale_type, out_type, relu, reserved;
+} dce_matmul_desc;
+int  dce_matmul(int device_id, void* hip_stream, const dce_matmul_desc* d);
+
+/* Rows in the order of their group: ids (n) int32 or int64 (id_bytes 4 | 8) -> offsets (groups + 1), order (n: the row at every place, rows of a group in
+ * their own order, -1 behind the last group), place (n: the place of every row; -1 for an id outside [0, groups), which belongs to no group).  work:
+ * dce_group_rows_work(n, groups) int32 of device memory (may be 0), used by this call alone until it has run. */
+int64_t dce_group_rows_work(int64_t n, int groups);
+int  dce_group_rows(int device_id, void* hip_stream, const void* ids, int id_bytes, int64_t n, int groups,
+                    int32_t* offsets, int32_t* order, int32_t* place, int32_t* work);
+
+/* torch.max(output, 1) + decimal2binary (src/inference_one_seq.py:25-27) on (rows, 16) logits picked by index (n; NULL: rows 0 .. n - 1): logits_out
+ * (n, 16), pred (n), contacts (n, 4), any may be NULL.  An index outside [0, rows): NaN logits, and so class 0. */
+int  dce_decide(int device_id, void* hip_stream, const float* logits, int64_t rows, const int32_t* index, int64_t n,
+                float* logits_out, int32_t* pred, uint8_t* contacts);
+
 #ifdef __cplusplus
 }
 #endif

@@ -44,7 +44,7 @@ with tempfile.TemporaryDirectory() as d:
     procs = []
     for s in (only or build.SOURCES):
         out = os.path.join(d, s + ".s")
-        procs.append((s, out, subprocess.Popen([build._hipcc(), *build.CFLAGS, *flags, "--cuda-device-only", "-S", os.path.join(build.CSRC, s), "-o", out],
+        procs.append((s, out, subprocess.Popen([build._hipcc(), *build.CFLAGS, *build.file_flags(s), *flags, "--cuda-device-only", "-S", os.path.join(build.CSRC, s), "-o", out],
                                                 stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)))
     for s, out, p in procs:
         assert p.wait() == 0, s
