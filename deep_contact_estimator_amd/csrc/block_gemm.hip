@@ -5,8 +5,8 @@
 //
 // The inner sums run on the matrix pipe in fp32; fp32 scales multiply a block's sum on the vector pipe (one fma a value), e8m0 scales are operands
 // of the 8-bit matrix instruction itself.  One matrix instruction of 16 x 16 x 128 covers a block along K; the bf16 form takes two of 16 x 16 x 32 for the
-// same 128 bytes of a row, so one layout in LDS serves both: rows of 128 bytes, eight 16-byte chunks, chunk c of row r in slot c ^ (r & 7) -- the
-// eight rows that one access serves lie in eight different slots.
+// same 128 bytes of a row, so one layout in LDS serves both: rows of 128 bytes, eight 16-byte chunks, chunk c of row r in slot c ^ ((r >> 1) & 7)
+// -- of the sixteen rows that one access serves, two share a line of 256 bytes and the pairs lie in eight different slots.
 //
 // The weights are the instruction's FIRST operand: a lane then holds four neighbouring columns of one row of y (one activation scale a lane, vector
 // stores).  Lane l: row l & 15 of either operand, chunks l >> 4 and (l >> 4) + 4.
@@ -55,7 +55,8 @@ __device__ __forceinline__ long long source_row(const ProductArgs& p, int j, int
 }
 
 // chunk c of row r of a tile in LDS
-__device__ __forceinline__ i32x4 chunk(const char* lds, int r, int c) { return *reinterpret_cast<const i32x4*>(lds + r * KROW + ((c ^ (r & 7)) * 16)); }
+__device__ __forceinline__ int slot_of(int r, int c) { return r * KROW + ((c ^ ((r >> 1) & 7)) * 16); }
+__device__ __forceinline__ i32x4 chunk(const char* lds, int r, int c) { return *reinterpret_cast<const i32x4*>(lds + slot_of(r, c)); }
 
 // 32 e4m3 values -> fp16, without error
 __device__ __forceinline__ void to_f16(i32x4 v, f16x8& lo, f16x8& hi)
@@ -84,12 +85,13 @@ template <> struct Frag<IN_BF16, true> : Frag<IN_BF16, false> {};
 // The scales of a step for a lane's row of x and a block of columns.  fp32: their product.  e8m0: the two bytes for the matrix instruction, or (EXACT) the
 // sum of the exponents; a byte of 255 is NaN there too.
 template <int IN, bool EXACT> struct Scale {
-    float s, start; int ew, ex;
-    __device__ __forceinline__ void set_f32(float w, float x) { s = w * x; }
-    __device__ __forceinline__ void set_e8(int w, int x)
+    float s, start; int e;
+    // v: the product of the fp32 scales, or the bytes (weights << 8 | x)
+    __device__ __forceinline__ void set(unsigned v)
     {
-        if (EXACT) { ew = w + x - 254; start = w == 255 || x == 255 ? __builtin_nanf("") : 0.f; }
-        else { ew = w; ex = x; }
+        if (IN == IN_F8_F32) s = __uint_as_float(v);
+        else if (EXACT) { const int w = (int)(v >> 8), x = (int)(v & 255); e = w + x - 254; start = w == 255 || x == 255 ? __builtin_nanf("") : 0.f; }
+        else e = (int)v;
     }
 };
 
@@ -100,27 +102,41 @@ template <int IN, bool EXACT> struct Scale {
 // of the rounding to bf16 (1.7e-3) and less still of that to e4m3, so results in those types take it.  fp32 results would be a hundred times worse
 // than their type: they take the operands as fp16 (every e4m3 number is one) through the fp16 instruction, at half the rate, whose sums of 32 products
 // are good to 1e-8.
-template <int IN, bool EXACT>
-__device__ __forceinline__ void mac(f32x4& acc, const Frag<IN, EXACT>& w, const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
+//
+// One row of blocks at a time: instructions that add to the same sums are as far apart as the row is long (a dependent one waits for its predecessor).
+template <int IN, bool EXACT, int NT>
+__device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> (&w)[NT], const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
 {
     if constexpr (IN == IN_BF16) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.c0), __builtin_bit_cast(bf16x8, x.c0), acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.c1), __builtin_bit_cast(bf16x8, x.c1), acc, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j].c0), __builtin_bit_cast(bf16x8, x.c0), acc[j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j].c1), __builtin_bit_cast(bf16x8, x.c1), acc[j], 0, 0, 0);
     } else if constexpr (EXACT) {
         const float z = IN == IN_F8_E8 ? sc.start : 0.f;
-        f32x4 part = {z, z, z, z};
+        f32x4 part[NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.h[i], x.h[i], part, 0, 0, 0);
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = IN == IN_F8_E8 ? acc[i] + ldexpf(part[i], sc.ew) : fmaf(part[i], sc.s, acc[i]);
+            for (int j = 0; j < NT; ++j) part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j].h[k], x.h[k], k ? part[j] : f32x4{z, z, z, z}, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = IN == IN_F8_E8 ? acc[j][i] + ldexpf(part[j][i], sc.e) : fmaf(part[j][i], sc.s, acc[j][i]);
     } else {
-        const i32x8 wv = __builtin_shufflevector(w.c0, w.c1, 0, 1, 2, 3, 4, 5, 6, 7), xv = __builtin_shufflevector(x.c0, x.c1, 0, 1, 2, 3, 4, 5, 6, 7);
-        if constexpr (IN == IN_F8_E8) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc, 0, 0, 0, sc.ew, 0, sc.ex);
-        else {
-            const f32x4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 127, 0, 127);
+        const i32x8 xv = __builtin_shufflevector(x.c0, x.c1, 0, 1, 2, 3, 4, 5, 6, 7);
+        f32x4 part[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(part[i], sc.s, acc[i]);
+        for (int j = 0; j < NT; ++j) {
+            const i32x8 wv = __builtin_shufflevector(w[j].c0, w[j].c1, 0, 1, 2, 3, 4, 5, 6, 7);
+            if constexpr (IN == IN_F8_E8) acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[j], 0, 0, 1, sc.e, 0, sc.e);      // (byte 1 the weights', byte 0 x's)
+            else part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 127, 0, 127);
         }
+        if constexpr (IN == IN_F8_F32)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[j][i], sc.s, acc[j][i]);
     }
 }
 
@@ -199,9 +215,9 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
     const long long mine = source_row(p, first + wave * 16 + r, end);         // the row whose scales this lane applies
     const long long sb0 = g * p.sb_group + (long long)tn * p.sb_row;
 
-    f32x4 acc[8];
+    f32x4 acc[2][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 8; ++i) acc[i >> 2][i & 3] = f32x4{0.f, 0.f, 0.f, 0.f};
     i32x4 next[CH];
     if (steps) fetch(0, next);
     for (int s = 0; s < steps; ++s) {
@@ -209,34 +225,35 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int lr = (int)(threadIdx.x >> 3) + 32 * i;
-            *reinterpret_cast<i32x4*>(lds + lr * KROW + ((c8 ^ (lr & 7)) * 16)) = next[i];
+            *reinterpret_cast<i32x4*>(lds + slot_of(lr, c8)) = next[i];
         }
         __syncthreads();
         Scale<IN, EXACT> sc;
-        if constexpr (IN == IN_F8_F32) sc.set_f32(static_cast<const float*>(p.sb)[sb0 + s], mine >= 0 ? static_cast<const float*>(p.sa)[s * p.sa_block + mine] : 1.f);
-        if constexpr (IN == IN_F8_E8) sc.set_e8(static_cast<const unsigned char*>(p.sb)[sb0 + s], mine >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine] : 127);
+        if constexpr (IN == IN_F8_F32) sc.set(__float_as_uint(static_cast<const float*>(p.sb)[sb0 + s] * (mine >= 0 ? static_cast<const float*>(p.sa)[s * p.sa_block + mine] : 1.f)));
+        if constexpr (IN == IN_F8_E8) sc.set((unsigned)static_cast<const unsigned char*>(p.sb)[sb0 + s] << 8 | (mine >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine] : 127u));
         if (s + 1 < steps) fetch(s + 1, next);
         const int xr = wave * 16 + r;
-        Frag<IN, EXACT> x, w;
+        Frag<IN, EXACT> x;
         x.set(chunk(lds, xr, q), chunk(lds, xr, q + 4));
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-            const int wr = BM + nt * 16 + r;
-            w.set(chunk(lds, wr, q), chunk(lds, wr, q + 4));
-            mac<IN, EXACT>(acc[nt], w, x, sc);
+        for (int h = 0; h < 2; ++h) {
+            Frag<IN, EXACT> w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const int wr = BM + (h * 4 + j) * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4)); }
+            mac_row<IN, EXACT, 4>(acc[h], w, x, sc);
         }
     }
     const int j = first + wave * 16 + r;
     const float* bias = p.bias ? p.bias + g * p.bias_group : nullptr;
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt) acc[nt] = finish(p, acc[nt], bias, n0 + nt * 16 + q * 4);
+    for (int nt = 0; nt < 8; ++nt) acc[nt >> 2][nt & 3] = finish(p, acc[nt >> 2][nt & 3], bias, n0 + nt * 16 + q * 4);
     float inv = 1.f;
     if constexpr (OUT == OUT_E4M3) {
         float most = 0.f;                                                     // (columns from n on hold bias-free zeros of zero rows)
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) most = fmaxf(most, finite_abs(acc[nt][i]));
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, finite_abs(acc[nt >> 2][nt & 3][i]));
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
         const int e = block_exponent(most);
@@ -251,31 +268,407 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt) {
         const int c = n0 + nt * 16 + q * 4;
-        if (c < p.n) store4<OUT>(p, j, c, acc[nt] * inv, wide);
+        if (c < p.n) store4<OUT>(p, j, c, acc[nt >> 2][nt & 3] * inv, wide);
     }
 }
 
+// ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave.  Both panels of a step
+//      come by LDS-DMA into one of two buffers while the matrix pipe works on the other; one barrier a step.
+__device__ __attribute__((aligned(16))) const char zero16[16] = {};
+
+// 64 lanes x 16 bytes from the lanes' addresses to LDS at `lds` (+ lane * 16)
+__device__ __forceinline__ void dma16(const char* from, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(lds) : "memory");
+}
+// ... from `from` + the lanes' offsets
+__device__ __forceinline__ void dma16s(const char* from, unsigned at, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" :: "s"(from), "v"(at), "s"(lds) : "memory");
+}
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p; }
+
+template <int WM_, int WN_, int MT_, int NT_> struct Tile {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;              // waves along the rows / the columns; blocks of 16 a wave
+    static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int BUF = (BM + BN) * KROW, PIECES = BUF / 1024 / WAVES;   // a piece: eight rows, one instruction
+    static constexpr int CB = BN / BLK, SCALES = BM * CB;
+    static constexpr int LDS = 2 * BUF + 2 * SCALES * 4;
+    static_assert(BUF % (1024 * WAVES) == 0 && BM % 8 == 0 && BN % BLK == 0 && SCALES <= THREADS, "tile");
+};
+
+// What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
+// sixteen rows at a time round in its own corner of LDS (a lane holds four columns of a row, a store takes neighbouring lanes along a row).
+template <int IN, int OUT, class T>
+__device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T::MT][T::NT], char* smem, int g, int first, int end, int n0, int wave, int lane)
+{
+    constexpr int SZ = OUT == OUT_F32 ? 4 : OUT == OUT_BF16 ? 2 : 1, ROW = T::NT * 16 * SZ, PITCH = ROW + 16, PER = BLK / (T::NT * 16);
+    const int r = lane & 15, q = lane >> 4, wm = (wave / T::WN) * T::MT * 16, wn = (wave % T::WN) * T::NT * 16;
+    float* const most = reinterpret_cast<float*>(smem);                       // [wave column][row]
+    char* const turn = smem + (OUT == OUT_E4M3 ? T::WN * T::BM * 4 : 0) + wave * 16 * PITCH;
+    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH <= T::LDS, "LDS");
+    f32x4 bias[T::NT];
+#pragma unroll
+    for (int u = 0; u < T::NT; ++u)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int c = n0 + wn + u * 16 + q * 4 + v;
+            bias[u][v] = p.bias && c < p.n ? p.bias[g * p.bias_group + c] : 0.f;
+        }
+    float top[T::MT];
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i) {
+        const bool none = p.index && source_row(p, first + wm + i * 16 + r, end) < 0;
+        top[i] = 0.f;
+#pragma unroll
+        for (int u = 0; u < T::NT; ++u)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                float y = (none ? 0.f : acc[i][u][v]) + bias[u][v];
+                if (p.relu) y = y < 0.f ? 0.f : y;                            // (NaN stays)
+                acc[i][u][v] = y;
+                if (OUT == OUT_E4M3 && n0 + wn + u * 16 + q * 4 + v < p.n) top[i] = fmaxf(top[i], finite_abs(y));
+            }
+        if constexpr (OUT == OUT_E4M3) {
+            top[i] = fmaxf(top[i], __shfl_xor(top[i], 16));
+            top[i] = fmaxf(top[i], __shfl_xor(top[i], 32));
+            if (q == 0) most[(wave % T::WN) * T::BM + wm + i * 16 + r] = top[i];
+        }
+    }
+    if constexpr (OUT == OUT_E4M3) {
+        __syncthreads();
+        const int cb = (n0 + wn) / BLK;
+#pragma unroll
+        for (int i = 0; i < T::MT; ++i) {
+            const int j = first + wm + i * 16 + r;
+            float t = 0.f;
+#pragma unroll
+            for (int u = 0; u < PER; ++u) t = fmaxf(t, most[((wave % T::WN) / PER * PER + u) * T::BM + wm + i * 16 + r]);
+            const int e = block_exponent(t);
+            const float inv = two_to(-e);
+#pragma unroll
+            for (int u = 0; u < T::NT; ++u) acc[i][u] *= inv;
+            if (q == 0 && j < end && (wave % T::WN) % PER == 0 && cb * BLK < p.n) {
+                if (IN == IN_F8_E8) static_cast<unsigned char*>(p.ys)[cb * p.ys_block + j] = (unsigned char)(e + 127);
+                else static_cast<float*>(p.ys)[cb * p.ys_block + j] = two_to(e);
+            }
+        }
+    }
+    const bool whole = wide_stores(p, 16) && n0 + wn + T::NT * 16 <= p.n;
+    const bool wide = wide_stores(p, 4 * SZ);
+    char* const y0 = p.y + (long long)(n0 + wn) * SZ;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i) {
+        const int j0 = first + wm + i * 16;
+        if (whole) {
+#pragma unroll
+            for (int u = 0; u < T::NT; ++u) {
+                char* at = turn + r * PITCH + (u * 16 + q * 4) * SZ;
+                if constexpr (OUT == OUT_F32) *reinterpret_cast<f32x4*>(at) = acc[i][u];
+                else if constexpr (OUT == OUT_BF16)
+                    *reinterpret_cast<uint2*>(at) = make_uint2(to_bf16(acc[i][u][0]) | (unsigned)to_bf16(acc[i][u][1]) << 16, to_bf16(acc[i][u][2]) | (unsigned)to_bf16(acc[i][u][3]) << 16);
+                else *reinterpret_cast<int*>(at) = to_e4m3x4(acc[i][u][0], acc[i][u][1], acc[i][u][2], acc[i][u][3]);
+            }
+            __builtin_amdgcn_wave_barrier();
+            constexpr int CH = ROW / 16;                                      // 16-byte pieces of a row
+#pragma unroll
+            for (int t = 0; t < CH * 16 / 64; ++t) {
+                const int row = (t * 64 + lane) / CH, c = (t * 64 + lane) % CH;
+                const i32x4 v = *reinterpret_cast<const i32x4*>(turn + row * PITCH + c * 16);
+                if (j0 + row < end) *reinterpret_cast<i32x4*>(y0 + (long long)(j0 + row) * p.y_row + c * 16) = v;
+            }
+            __builtin_amdgcn_wave_barrier();
+        } else if (j0 + r < end) {
+#pragma unroll
+            for (int u = 0; u < T::NT; ++u) {
+                const int c = n0 + wn + u * 16 + q * 4;
+                if (c < p.n) store4<OUT>(p, j0 + r, c, acc[i][u], wide);
+            }
+        }
+    }
+}
+
+template <int IN, int OUT, class T>
+__global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs p)
+{
+    constexpr bool EXACT = OUT == OUT_F32;
+    constexpr int BM = T::BM, BN = T::BN, MT = T::MT, NT = T::NT;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    unsigned* const scales = reinterpret_cast<unsigned*>(smem + 2 * T::BUF);  // [2][column block][row]
+    // neighbouring tiles on one XCD (workgroups go round the eight of them), columns first
+    const unsigned per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    int g, first, end;
+    const int tn = (int)(id % (unsigned)p.tiles_n);
+    if (!find_tile(p, BM, (int)(id / (unsigned)p.tiles_n), g, first, end)) return;
+    const int n0 = tn * BN, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    const int wm = (wave / T::WN) * MT * 16, wn = (wave % T::WN) * NT * 16;
+    const int steps = (p.kbytes + KROW - 1) / KROW;
+
+    const char* from[T::PIECES];
+    int col16[T::PIECES];
+#pragma unroll
+    for (int i = 0; i < T::PIECES; ++i) {
+        const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3);
+        col16[i] = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
+        if (i * T::WAVES * 8 < BM) {                                          // (a piece lies in one panel: BM is a multiple of a round's rows)
+            const long long s = source_row(p, first + lr, end);
+            from[i] = p.a + (s < 0 ? 0 : s) * p.a_row + col16[i];             // rows without a source: any row, taken out at the end
+        } else {
+            const int c = n0 + lr - BM;
+            from[i] = p.b + g * p.b_group + (long long)(c < p.n ? c : p.n - 1) * p.b_row + col16[i];
+        }
+    }
+    static_assert(BM % (T::WAVES * 8) == 0, "a round of pieces lies in one panel");
+    const unsigned lds0 = lds_addr(smem);
+    auto bring = [&](int s) {
+        const bool last = (s + 1) * KROW > p.kbytes;                          // a step that K ends inside: chunks behind it come from a zero
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i) {
+            const char* a = from[i];
+            if (last && s * KROW + col16[i] >= p.kbytes) a = zero16;
+            dma16(a, lds0 + (s & 1) * T::BUF + (i * T::WAVES + wave) * 1024);
+            from[i] += KROW;
+        }
+    };
+    // the scale of row `tid` % BM and column block tid / BM, a step ahead in a register
+    long long sa_at = 0, sb_at = 0;
+    if (IN != IN_BF16 && tid < T::SCALES) {
+        const long long s = source_row(p, first + tid % BM, end);
+        sa_at = s < 0 ? 0 : s;
+        const int u = (n0 + BLK * (tid / BM)) / BLK, last = (p.n - 1) / BLK;
+        sb_at = g * p.sb_group + (long long)(u < last ? u : last) * p.sb_row;
+    }
+    unsigned s_x = 0, s_w = 0;
+    auto bring_scale = [&](int s) {
+        if (IN == IN_BF16 || tid >= T::SCALES) return;
+        if (IN == IN_F8_F32) { s_x = static_cast<const unsigned*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned*>(p.sb)[sb_at + s]; }
+        else { s_x = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned char*>(p.sb)[sb_at + s]; }
+    };
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bring_scale(0);
+    bring(0);
+    for (int s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (IN != IN_BF16 && tid < T::SCALES)
+            scales[(s & 1) * T::SCALES + tid] = IN == IN_F8_F32 ? __float_as_uint(__uint_as_float(s_w) * __uint_as_float(s_x)) : s_w << 8 | s_x;
+        __syncthreads();                                                      // the step's panels are there, the other buffer has been read
+        if (s + 1 < steps) { bring_scale(s + 1); bring(s + 1); }
+        const char* xa = smem + (s & 1) * T::BUF;
+        const char* wa = xa + BM * KROW;
+        Frag<IN, EXACT> w[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            Frag<IN, EXACT> x;
+            x.set(chunk(xa, wm + i * 16 + r, q), chunk(xa, wm + i * 16 + r, q + 4));
+            Scale<IN, EXACT> sc;
+            if (IN != IN_BF16) sc.set(scales[(s & 1) * T::SCALES + (wn / BLK) * BM + wm + i * 16 + r]);
+            mac_row<IN, EXACT, NT>(acc[i], w, x, sc);
+        }
+    }
+    __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
+    store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
+}
+
+// ---- the kernel for chip-filling products (K a multiple of 128 bytes, operands within 4 GB): eight waves in two groups that are half a phase apart.
+//
+// Waves w and w + 4 share a SIMD.  While one group's phase is sixteen blocks' matrix instructions a wave, the other group's is reads of fragments from LDS and
+// waits: the matrix pipe passes from one group to the other without a pause, and no wave waits for LDS with the pipe idle.  A step of group 0 is
+// La Ma (Lb Mb), L = some rows of blocks read, M = multiplied; group 1 runs the same one phase later; a barrier ends every phase.  Step s + 1's
+// panels are asked for at phase 2H s of H = MT / XG pairs (its buffer was last read in the phase before) and have landed before phase 2H (s + 1).
+template <int IN, int OUT, class T>
+__global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductArgs p)
+{
+    constexpr bool EXACT = OUT == OUT_F32;
+    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, XG = EXACT && IN != IN_BF16 ? 2 : 4, H = MT / XG;   // (e4m3 as fp16 takes twice the registers)
+    static_assert(T::WM == 2 && T::WN == 4 && MT % XG == 0 && BM % (T::WAVES * 8) == 0, "tile");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    unsigned* const scales = reinterpret_cast<unsigned*>(smem + 2 * T::BUF);  // [2][column block][row]
+    const unsigned per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    int g, first, end;
+    const int tn = (int)(id % (unsigned)p.tiles_n);
+    if (!find_tile(p, BM, (int)(id / (unsigned)p.tiles_n), g, first, end)) return;
+    const int n0 = tn * T::BN, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    const int grp = wave >> 2, wm = grp * MT * 16, wn = (wave & 3) * NT * 16;
+    const int steps = p.kbytes / KROW;
+
+    unsigned from[T::PIECES];                                                 // from the step's column of a, of the group's b
+    constexpr int PA = BM / (T::WAVES * 8);
+#pragma unroll
+    for (int i = 0; i < T::PIECES; ++i) {
+        const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3), col = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
+        unsigned row;
+        if (i < PA) { const long long s = source_row(p, first + lr, end); row = (unsigned)(s < 0 ? 0 : s) * (unsigned)p.a_row; }
+        else { const int c = n0 + lr - BM; row = (unsigned)(c < p.n ? c : p.n - 1) * (unsigned)p.b_row; }
+        asm volatile("" : "+v"(row));                                         // (a product and a sum of 32 bits: not the instruction whose result fills two registers)
+        from[i] = row + col;
+    }
+    const unsigned lds0 = lds_addr(smem);
+    const char* const b0 = p.b + g * p.b_group;
+    long long sa_at = 0, sb_at = 0;
+    if (IN != IN_BF16 && tid < T::SCALES) {
+        const long long s = source_row(p, first + tid % BM, end);
+        sa_at = s < 0 ? 0 : s;
+        const int u = (n0 + BLK * (tid / BM)) / BLK, last = (p.n - 1) / BLK;
+        sb_at = g * p.sb_group + (long long)(u < last ? u : last) * p.sb_row;
+    }
+    unsigned s_x = 0, s_w = 0;
+    auto bring = [&](int s) {
+        const char* const ak = p.a + (long long)s * KROW;
+        const char* const bk = b0 + (long long)s * KROW;
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i) dma16s(i < PA ? ak : bk, from[i], lds0 + (s & 1) * T::BUF + (i * T::WAVES + wave) * 1024);
+        if (IN == IN_BF16 || tid >= T::SCALES) return;
+        if (IN == IN_F8_F32) { s_x = static_cast<const unsigned*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned*>(p.sb)[sb_at + s]; }
+        else { s_x = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned char*>(p.sb)[sb_at + s]; }
+    };
+    auto landed = [&](int s) {                                                // this wave's pieces and scales of step s are in LDS
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (IN != IN_BF16 && tid < T::SCALES)
+            scales[(s & 1) * T::SCALES + tid] = IN == IN_F8_F32 ? __float_as_uint(__uint_as_float(s_w) * __uint_as_float(s_x)) : s_w << 8 | s_x;
+    };
+    auto phase_end = [&] {                                                    // (matrix instructions touch no memory: the scheduling barriers keep them in their phase)
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bring(0);
+    landed(0);
+    phase_end();
+    if (grp == 1) {
+        if (steps > 1) bring(1);
+        phase_end();
+    }
+    for (int s = 0; s < steps; ++s) {
+        const char* const xa = smem + (s & 1) * T::BUF;
+        const char* const wa = xa + BM * KROW;
+        Frag<IN, EXACT> w[NT];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            // ---- L
+            if (h == 0) {
+                if (grp == 0 && s + 1 < steps) bring(s + 1);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4));
+            }
+            Frag<IN, EXACT> x[XG];
+            unsigned sv[XG];
+#pragma unroll
+            for (int i = 0; i < XG; ++i) {
+                const int row = wm + (h * XG + i) * 16 + r;
+                x[i].set(chunk(xa, row, q), chunk(xa, row, q + 4));
+                if (IN != IN_BF16) sv[i] = scales[(s & 1) * T::SCALES + (wn / BLK) * BM + row];
+            }
+            if (h == H - 1 && grp == 1 && s + 1 < steps) landed(s + 1);
+            phase_end();
+            // ---- M
+            if (h == H - 1 && grp == 1 && s + 2 < steps) bring(s + 2);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int i = 0; i < XG; ++i) {
+                Scale<IN, EXACT> sc;
+                if (IN != IN_BF16) sc.set(sv[i]);
+                mac_row<IN, EXACT, NT>(acc[h * XG + i], w, x[i], sc);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            if (h < H - 1) {                                                  // (the compiler would put them off to the end of the step)
+#pragma unroll
+                for (int i = 0; i < XG; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) asm volatile("" :: "v"(acc[h * XG + i][j]));
+            }
+            if (h == H - 1 && grp == 0 && s + 1 < steps) landed(s + 1);
+            phase_end();
+        }
+    }
+    if (grp == 0) phase_end();
+    store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
+}
+
 namespace {
-template <int IN>
-hipError_t launch_any(ProductArgs p, int out, hipStream_t st)
+
+long long row_tiles(const ProductArgs& p, int bm)                             // at most: a group of rows ends inside a tile
+{
+    return p.offsets ? (long long)p.m / bm + (p.groups < p.m ? p.groups : p.m) : ((long long)p.m + bm - 1) / bm;
+}
+
+template <int IN, int OUT>
+hipError_t launch_any(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + 127) / 128;
-    const long long tiles_m = p.offsets ? (long long)p.m / 64 + (p.groups < p.m ? p.groups : p.m) : ((long long)p.m + 63) / 64;
-    if (tiles_m * p.tiles_n > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)(tiles_m * p.tiles_n));
-    if (out == OUT_F32) product_any_kernel<IN, OUT_F32><<<grid, 256, 0, st>>>(p);
-    else if (out == OUT_BF16) product_any_kernel<IN, OUT_BF16><<<grid, 256, 0, st>>>(p);
-    else if constexpr (IN != IN_BF16) product_any_kernel<IN, OUT_E4M3><<<grid, 256, 0, st>>>(p);
-    else return hipErrorInvalidValue;
+    const long long tiles = row_tiles(p, 64) * p.tiles_n;
+    if (tiles > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    product_any_kernel<IN, OUT><<<(unsigned)tiles, 256, 0, st>>>(p);
     return hipGetLastError();
 }
+
+template <int IN, int OUT, class T>
+hipError_t launch_tile(ProductArgs p, hipStream_t st)
+{
+    p.tiles_n = (p.n + T::BN - 1) / T::BN;
+    const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
+    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(product_tile_kernel<IN, OUT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (once != hipSuccess) return once;
+    product_tile_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int IN, int OUT, class T>
+hipError_t launch_phased(ProductArgs p, hipStream_t st)
+{
+    p.tiles_n = (p.n + T::BN - 1) / T::BN;
+    const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
+    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(product_phased_kernel<IN, OUT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (once != hipSuccess) return once;
+    product_phased_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int IN, int OUT>
+hipError_t launch_out(const ProductArgs& p, hipStream_t st)
+{
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
+    if (!aligned || p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
+    using T256 = Tile<2, 4, 8, 4>;
+    using T128W = Tile<2, 4, 4, 4>;
+    using T128 = Tile<2, 2, 4, 4>;
+    const bool near = p.kbytes % KROW == 0 && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);
+    if constexpr (IN == IN_BF16 || OUT != OUT_F32)
+        if (near && row_tiles(p, 256) * ((p.n + 255) / 256) >= 256) return launch_phased<IN, OUT, T256>(p, st);
+    if (near && row_tiles(p, 128) * ((p.n + 255) / 256) >= 256) return launch_phased<IN, OUT, T128W>(p, st);
+    return launch_tile<IN, OUT, T128>(p, st);
+}
+
+template <int IN>
+hipError_t launch_in(const ProductArgs& p, int out, hipStream_t st)
+{
+    if (out == OUT_F32) return launch_out<IN, OUT_F32>(p, st);
+    if (out == OUT_BF16) return launch_out<IN, OUT_BF16>(p, st);
+    if constexpr (IN != IN_BF16) return launch_out<IN, OUT_E4M3>(p, st);
+    return hipErrorInvalidValue;
+}
+
 }  // namespace
 
 hipError_t launch_product(const ProductArgs& p, int in, int out, hipStream_t st)
 {
-    if (in == IN_BF16) return launch_any<IN_BF16>(p, out, st);
-    if (in == IN_F8_F32) return launch_any<IN_F8_F32>(p, out, st);
-    return launch_any<IN_F8_E8>(p, out, st);
+    if (in == IN_BF16) return launch_in<IN_BF16>(p, out, st);
+    if (in == IN_F8_F32) return launch_in<IN_F8_F32>(p, out, st);
+    return launch_in<IN_F8_E8>(p, out, st);
 }
 
 }  // namespace dce

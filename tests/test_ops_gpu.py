@@ -174,7 +174,8 @@ def operands(ops, m, n, k, scale, seed, groups=0):
 
 
 SIZES = [(1, 1, 1), (1, 2048, 4736), (2, 16, 128), (15, 17, 129), (16, 128, 256), (17, 130, 127), (30, 512, 2048), (33, 250, 1000), (64, 64, 64), (65, 129, 100), (129, 384, 48),
-         (300, 1000, 384), (257, 256, 1419), (700, 512, 512), (1300, 2048, 640)]
+         (300, 1000, 384), (257, 256, 1419), (700, 512, 512), (1300, 2048, 640),
+         (4100, 4200, 256), (4200, 2050, 384), (4099, 4104, 144), (8200, 2000, 128)]          # (enough tiles to fill the chip)
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, F8])
@@ -306,7 +307,7 @@ def plain_grouped(a, sa, b, sb, bias, counts, index, relu, coarse=False):
 @pytest.mark.parametrize("form", ["bf16", E8, torch.float32])
 @pytest.mark.parametrize("m, n, k, groups, kind", [
     (1, 16, 64, 1, "even"), (8, 512, 256, 8, "even"), (5, 40, 100, 9, "ragged"), (30, 128, 512, 4, "ragged"), (64, 130, 129, 3, "ragged"), (65, 96, 200, 2, "one"), (100, 33, 65, 7, "one"),
-    (257, 512, 384, 5, "ragged"), (777, 200, 320, 64, "ragged"), (900, 256, 256, 100, "ragged"), (1500, 320, 512, 3, "ragged"), (40, 16, 48, 1024, "ragged")])
+    (257, 512, 384, 5, "ragged"), (777, 200, 320, 64, "ragged"), (900, 256, 256, 100, "ragged"), (1500, 320, 512, 3, "ragged"), (9000, 2100, 256, 6, "ragged"), (5000, 1500, 384, 7, "ragged"), (5000, 1500, 400, 7, "ragged"), (40, 16, 48, 1024, "ragged")])
 def test_matmul_grouped(ops, m, n, k, groups, kind, form):
     counts = counts_of(kind, m, groups, m)
     for gather, out, relu in ((False, torch.float32, False), (True, torch.bfloat16, True)):
