@@ -18,30 +18,42 @@ namespace {
 
 __device__ __forceinline__ int clamp_to(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
 
-// The group, first row and end of row tile t (tiles of bm rows, counted group by group).  Offsets are held inside [0, m] whatever they say.
-// Every wave works it out for itself: 64 groups a step, tiles counted by a scan over the lanes.
-__device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, int t, int& g, int& first, int& end)
+struct Place { int g, first, end, tn; };      // a tile: its group, its first row and the group's end, its column tile
+
+// The tile of this workgroup.  Row tiles are counted group by group (offsets are held inside [0, m] whatever they say) and only here: the host knows no
+// more than a bound.  Workgroups go round the eight XCDs, so workgroup 8 i + x takes the i-th tile of the x-th eighth of those that there are: neighbours
+// share an L2, columns first.  64 groups a step, tiles counted by a scan over the lanes; every wave does it for itself.
+__device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, Place& at)
 {
-    if (!p.offsets) { g = 0; first = t * bm; end = p.m; return first < p.m; }
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int base = 0; base < p.groups; base += 64) {
-        int lo = 0, hi = 0;
+    int lo = 0, hi = p.m, tiles = 0, sum = 0;
+    auto scan = [&](int base) {
+        lo = hi = 0;
         if (base + lane < p.groups) { lo = clamp_to(p.offsets[base + lane], p.m); hi = clamp_to(p.offsets[base + lane + 1], p.m); }
-        const int tiles = hi > lo ? (hi - lo + bm - 1) / bm : 0;
-        int sum = tiles;
+        sum = tiles = hi > lo ? (hi - lo + bm - 1) / bm : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(sum, d); if (lane >= d) sum += o; }
-        const int total = __builtin_amdgcn_readlane(sum, 63);
-        if (t < before + total) {
+        return __builtin_amdgcn_readlane(sum, 63);
+    };
+    int total = 0;
+    if (!p.offsets) total = (p.m + bm - 1) / bm;
+    else for (int base = 0; base < p.groups; base += 64) total += scan(base);
+    const unsigned all = (unsigned)total * (unsigned)p.tiles_n, per = (all + 7) >> 3, slot = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + slot;
+    if (slot >= per || id >= all) return false;
+    const int t = (int)(id / (unsigned)p.tiles_n);
+    at.tn = (int)(id % (unsigned)p.tiles_n);
+    if (!p.offsets) { at.g = 0; at.first = t * bm; at.end = p.m; return true; }
+    int before = 0;
+    for (int base = 0; base < p.groups; base += 64) {
+        const int here = p.groups <= 64 ? total : scan(base);
+        if (t < before + here) {
             const int w = __builtin_ctzll(__ballot(before + sum > t));
-            const int at = t - (before + __builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(tiles, w));
-            g = base + w;
-            first = __builtin_amdgcn_readlane(lo, w) + at * bm;
-            end = __builtin_amdgcn_readlane(hi, w);
+            at.g = base + w;
+            at.first = __builtin_amdgcn_readlane(lo, w) + (t - (before + __builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(tiles, w))) * bm;
+            at.end = __builtin_amdgcn_readlane(hi, w);
             return true;
         }
-        before += total;
+        before += here;
     }
     return false;
 }
@@ -85,13 +97,13 @@ template <> struct Frag<IN_BF16, true> : Frag<IN_BF16, false> {};
 // The scales of a step for a lane's row of x and a block of columns.  fp32: their product.  e8m0: the two bytes for the matrix instruction, or (EXACT) the
 // sum of the exponents; a byte of 255 is NaN there too.
 template <int IN, bool EXACT> struct Scale {
-    float s, start; int e;
-    // v: the product of the fp32 scales, or the bytes (weights << 8 | x)
-    __device__ __forceinline__ void set(unsigned v)
+    float s, start; int e, ew, ex;
+    // of the weights' block and of x's row: fp32 numbers, or bytes
+    __device__ __forceinline__ void set(unsigned w, unsigned x)
     {
-        if (IN == IN_F8_F32) s = __uint_as_float(v);
-        else if (EXACT) { const int w = (int)(v >> 8), x = (int)(v & 255); e = w + x - 254; start = w == 255 || x == 255 ? __builtin_nanf("") : 0.f; }
-        else e = (int)v;
+        if (IN == IN_F8_F32) s = __uint_as_float(w) * __uint_as_float(x);
+        else if (EXACT) { e = (int)(w + x) - 254; start = w == 255 || x == 255 ? __builtin_nanf("") : 0.f; }
+        else { ew = (int)w; ex = (int)x; }
     }
 };
 
@@ -129,7 +141,7 @@ __device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> 
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const i32x8 wv = __builtin_shufflevector(w[j].c0, w[j].c1, 0, 1, 2, 3, 4, 5, 6, 7);
-            if constexpr (IN == IN_F8_E8) acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[j], 0, 0, 1, sc.e, 0, sc.e);      // (byte 1 the weights', byte 0 x's)
+            if constexpr (IN == IN_F8_E8) acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[j], 0, 0, 0, sc.ew, 0, sc.ex);
             else part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 127, 0, 127);
         }
         if constexpr (IN == IN_F8_F32)
@@ -193,9 +205,9 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
     constexpr int BM = 64, BN = 128, CH = (BM + BN) * 8 / 256;               // 16-byte chunks a thread brings each step
     constexpr bool EXACT = OUT == OUT_F32;
     __shared__ __attribute__((aligned(16))) char lds[(BM + BN) * KROW];
-    int g, first, end;
-    const int tn = (int)(blockIdx.x % (unsigned)p.tiles_n);
-    if (!find_tile(p, BM, (int)(blockIdx.x / (unsigned)p.tiles_n), g, first, end)) return;
+    Place at;
+    if (!find_tile(p, BM, at)) return;
+    const int g = at.g, first = at.first, end = at.end, tn = at.tn;
     const int n0 = tn * BN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const int steps = (p.kbytes + KROW - 1) / KROW;
 
@@ -229,8 +241,8 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
         }
         __syncthreads();
         Scale<IN, EXACT> sc;
-        if constexpr (IN == IN_F8_F32) sc.set(__float_as_uint(static_cast<const float*>(p.sb)[sb0 + s] * (mine >= 0 ? static_cast<const float*>(p.sa)[s * p.sa_block + mine] : 1.f)));
-        if constexpr (IN == IN_F8_E8) sc.set((unsigned)static_cast<const unsigned char*>(p.sb)[sb0 + s] << 8 | (mine >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine] : 127u));
+        if constexpr (IN == IN_F8_F32) sc.set(static_cast<const unsigned*>(p.sb)[sb0 + s], mine >= 0 ? static_cast<const unsigned*>(p.sa)[s * p.sa_block + mine] : 0x3f800000u);
+        if constexpr (IN == IN_F8_E8) sc.set(static_cast<const unsigned char*>(p.sb)[sb0 + s], mine >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine] : 127u);
         if (s + 1 < steps) fetch(s + 1, next);
         const int xr = wave * 16 + r;
         Frag<IN, EXACT> x;
@@ -286,6 +298,15 @@ __device__ __forceinline__ void dma16s(const char* from, unsigned at, unsigned l
 {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" :: "s"(from), "v"(at), "s"(lds) : "memory");
 }
+// ... 64 lanes x 4 bytes / 1 byte (widened to a word), a word a lane in LDS
+__device__ __forceinline__ void dma4s(const char* from, unsigned at, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %0" :: "s"(from), "v"(at), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma1s(const char* from, unsigned at, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %0" :: "s"(from), "v"(at), "s"(lds) : "memory");
+}
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p; }
 
 template <int WM_, int WN_, int MT_, int NT_> struct Tile {
@@ -293,7 +314,7 @@ template <int WM_, int WN_, int MT_, int NT_> struct Tile {
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BUF = (BM + BN) * KROW, PIECES = BUF / 1024 / WAVES;   // a piece: eight rows, one instruction
     static constexpr int CB = BN / BLK, SCALES = BM * CB;
-    static constexpr int LDS = 2 * BUF + 2 * SCALES * 4;
+    static constexpr int LDS = 2 * BUF + 2 * SCALES * 8;
     static_assert(BUF % (1024 * WAVES) == 0 && BM % 8 == 0 && BN % BLK == 0 && SCALES <= THREADS, "tile");
 };
 
@@ -394,12 +415,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs
     constexpr bool EXACT = OUT == OUT_F32;
     constexpr int BM = T::BM, BN = T::BN, MT = T::MT, NT = T::NT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    unsigned* const scales = reinterpret_cast<unsigned*>(smem + 2 * T::BUF);  // [2][column block][row]
-    // neighbouring tiles on one XCD (workgroups go round the eight of them), columns first
-    const unsigned per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    int g, first, end;
-    const int tn = (int)(id % (unsigned)p.tiles_n);
-    if (!find_tile(p, BM, (int)(id / (unsigned)p.tiles_n), g, first, end)) return;
+    uint2* const scales = reinterpret_cast<uint2*>(smem + 2 * T::BUF);        // [2][column block][row]: the weights', x's
+    Place at;
+    if (!find_tile(p, BM, at)) return;
+    const int g = at.g, first = at.first, end = at.end, tn = at.tn;
     const int n0 = tn * BN, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
     const int wm = (wave / T::WN) * MT * 16, wn = (wave % T::WN) * NT * 16;
     const int steps = (p.kbytes + KROW - 1) / KROW;
@@ -455,7 +474,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs
     for (int s = 0; s < steps; ++s) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (IN != IN_BF16 && tid < T::SCALES)
-            scales[(s & 1) * T::SCALES + tid] = IN == IN_F8_F32 ? __float_as_uint(__uint_as_float(s_w) * __uint_as_float(s_x)) : s_w << 8 | s_x;
+            scales[(s & 1) * T::SCALES + tid] = make_uint2(s_w, s_x);
         __syncthreads();                                                      // the step's panels are there, the other buffer has been read
         if (s + 1 < steps) { bring_scale(s + 1); bring(s + 1); }
         const char* xa = smem + (s & 1) * T::BUF;
@@ -468,7 +487,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs
             Frag<IN, EXACT> x;
             x.set(chunk(xa, wm + i * 16 + r, q), chunk(xa, wm + i * 16 + r, q + 4));
             Scale<IN, EXACT> sc;
-            if (IN != IN_BF16) sc.set(scales[(s & 1) * T::SCALES + (wn / BLK) * BM + wm + i * 16 + r]);
+            if (IN != IN_BF16) { const uint2 v = scales[(s & 1) * T::SCALES + (wn / BLK) * BM + wm + i * 16 + r]; sc.set(v.x, v.y); }
             mac_row<IN, EXACT, NT>(acc[i], w, x, sc);
         }
     }
@@ -476,62 +495,88 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
-// ---- the kernel for chip-filling products (K a multiple of 128 bytes, operands within 4 GB): eight waves in two groups that are half a phase apart.
+// ---- the kernel for chip-filling products (K a multiple of 128 bytes, operands within 4 GB): eight waves in two groups that are a phase apart.
 //
-// Waves w and w + 4 share a SIMD.  While one group's phase is sixteen blocks' matrix instructions a wave, the other group's is reads of fragments from LDS and
-// waits: the matrix pipe passes from one group to the other without a pause, and no wave waits for LDS with the pipe idle.  A step of group 0 is
-// La Ma (Lb Mb), L = some rows of blocks read, M = multiplied; group 1 runs the same one phase later; a barrier ends every phase.  Step s + 1's
-// panels are asked for at phase 2H s of H = MT / XG pairs (its buffer was last read in the phase before) and have landed before phase 2H (s + 1).
+// Waves w and w + 4 share a SIMD.  While one group's phase is its matrix instructions, the other group's is reads of fragments from LDS and waits: the
+// matrix pipe passes from one group to the other without a pause, and no wave waits for LDS with the pipe idle.  A step of group 0 is L0 M0 .. (of
+// H = MT / XG pairs; L: XG rows of blocks read, M: multiplied; L0 reads all of the weights' fragments too), from phase 2H s on; group 1 runs the same
+// one phase later; a barrier ends every phase.
+//
+// 64 KB a step and CU are 1 us of what L2 gives to all CUs at once (measured, 17 TB/s) and another half before the first of them is there, against 0.9 us
+// of matrix instructions: panels have to be asked for more than a step ahead.  256 x 256 tiles leave room for two buffers, so each part of a panel is
+// asked for as soon as its buffer has been read for the last time: step s + 2's weights at phase 4s + 2, group 0's rows at 4s + 3, group 1's at
+// 4s + 4.  128 x 256 tiles have three buffers: step s + 2 at phase 2H s.  Scales come the same way, a word a row.
+template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;
+    static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int BUF = (BM + BN) * KROW, PA = BM / 64, PB = BN / 64;   // pieces of eight rows a wave brings: of its group's rows, of the weights
+    static constexpr int SLOT = (BM + 64) * 4;                                // a step's scales: the rows', the column blocks'
+    static constexpr int LDS = NBUF * BUF + 4 * SLOT;
+    static_assert(WM == 2 && WN == 4 && BN / BLK <= 64 && (NBUF == 2 || NBUF == 3), "two groups of four waves");
+};
+
+template <int N> __device__ __forceinline__ void wait_all_but() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+
 template <int IN, int OUT, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductArgs p)
 {
     constexpr bool EXACT = OUT == OUT_F32;
     constexpr int BM = T::BM, MT = T::MT, NT = T::NT, XG = EXACT && IN != IN_BF16 ? 2 : 4, H = MT / XG;   // (e4m3 as fp16 takes twice the registers)
-    static_assert(T::WM == 2 && T::WN == 4 && MT % XG == 0 && BM % (T::WAVES * 8) == 0, "tile");
+    constexpr int PA = T::PA, PB = T::PB, PS = IN != IN_BF16, NBUF = T::NBUF;
+    static_assert(MT % XG == 0 && (NBUF == 3 || H == 2), "phases");
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    unsigned* const scales = reinterpret_cast<unsigned*>(smem + 2 * T::BUF);  // [2][column block][row]
-    const unsigned per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    int g, first, end;
-    const int tn = (int)(id % (unsigned)p.tiles_n);
-    if (!find_tile(p, BM, (int)(id / (unsigned)p.tiles_n), g, first, end)) return;
-    const int n0 = tn * T::BN, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
-    const int grp = wave >> 2, wm = grp * MT * 16, wn = (wave & 3) * NT * 16;
+    Place place;
+    if (!find_tile(p, BM, place)) return;
+    const int g = place.g, first = place.first, end = place.end, n0 = place.tn * T::BN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    const int grp = wave >> 2, w4 = wave & 3, wm = grp * MT * 16, wn = w4 * NT * 16;
     const int steps = p.kbytes / KROW;
 
-    unsigned from[T::PIECES];                                                 // from the step's column of a, of the group's b
-    constexpr int PA = BM / (T::WAVES * 8);
+    unsigned from[PA + PB];                                                   // from the step's column of a, of the group's b
 #pragma unroll
-    for (int i = 0; i < T::PIECES; ++i) {
-        const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3), col = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
+    for (int i = 0; i < PA + PB; ++i) {
+        const int lr = (i < PA ? grp * (BM / 16) + i * 4 + w4 : (i - PA) * 8 + wave) * 8 + (lane >> 3), col = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
         unsigned row;
         if (i < PA) { const long long s = source_row(p, first + lr, end); row = (unsigned)(s < 0 ? 0 : s) * (unsigned)p.a_row; }
-        else { const int c = n0 + lr - BM; row = (unsigned)(c < p.n ? c : p.n - 1) * (unsigned)p.b_row; }
+        else { const int c = n0 + lr; row = (unsigned)(c < p.n ? c : p.n - 1) * (unsigned)p.b_row; }
         asm volatile("" : "+v"(row));                                         // (a product and a sum of 32 bits: not the instruction whose result fills two registers)
         from[i] = row + col;
     }
     const unsigned lds0 = lds_addr(smem);
     const char* const b0 = p.b + g * p.b_group;
-    long long sa_at = 0, sb_at = 0;
-    if (IN != IN_BF16 && tid < T::SCALES) {
-        const long long s = source_row(p, first + tid % BM, end);
-        sa_at = s < 0 ? 0 : s;
-        const int u = (n0 + BLK * (tid / BM)) / BLK, last = (p.n - 1) / BLK;
-        sb_at = g * p.sb_group + (long long)(u < last ? u : last) * p.sb_row;
+    // group 0 brings the scales of 64 rows a wave, group 1 those of the column blocks (every wave the same ones)
+    constexpr int SZ = IN == IN_F8_F32 ? 4 : 1;
+    const char* s_from = nullptr;
+    long long s_step = 0;
+    unsigned s_at = 0, s_to = 0;
+    if (PS && grp == 0) {
+        const int lr = w4 * 64 % BM + lane;
+        const long long s = source_row(p, first + lr, end);
+        s_from = static_cast<const char*>(p.sa);
+        s_step = p.sa_block * SZ;
+        s_at = (unsigned)(s < 0 ? 0 : s) * SZ;
+        s_to = w4 * 64 % BM * 4;
+    } else if (PS) {
+        const int u = n0 / BLK + lane % (T::BN / BLK), last = (p.n - 1) / BLK;
+        s_from = static_cast<const char*>(p.sb) + (g * p.sb_group + (long long)(n0 / BLK) * p.sb_row) * SZ;
+        s_step = SZ;
+        s_at = (unsigned)((u < last ? u : last) - n0 / BLK) * (unsigned)(p.sb_row * SZ);
+        s_to = BM * 4;
     }
-    unsigned s_x = 0, s_w = 0;
-    auto bring = [&](int s) {
-        const char* const ak = p.a + (long long)s * KROW;
-        const char* const bk = b0 + (long long)s * KROW;
+    auto bring_a = [&](int s, int buf) {
+        const char* const k = p.a + (long long)s * KROW;
+        if constexpr (PS) {
+            const unsigned to = lds0 + NBUF * T::BUF + (s & 3) * T::SLOT + s_to;
+            if constexpr (SZ == 4) dma4s(s_from + s * s_step, s_at, to);
+            else dma1s(s_from + s * s_step, s_at, to);
+        }
 #pragma unroll
-        for (int i = 0; i < T::PIECES; ++i) dma16s(i < PA ? ak : bk, from[i], lds0 + (s & 1) * T::BUF + (i * T::WAVES + wave) * 1024);
-        if (IN == IN_BF16 || tid >= T::SCALES) return;
-        if (IN == IN_F8_F32) { s_x = static_cast<const unsigned*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned*>(p.sb)[sb_at + s]; }
-        else { s_x = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned char*>(p.sb)[sb_at + s]; }
+        for (int i = 0; i < PA; ++i) dma16s(k, from[i], lds0 + buf * T::BUF + (grp * (BM / 16) + i * 4 + w4) * 1024);
     };
-    auto landed = [&](int s) {                                                // this wave's pieces and scales of step s are in LDS
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (IN != IN_BF16 && tid < T::SCALES)
-            scales[(s & 1) * T::SCALES + tid] = IN == IN_F8_F32 ? __float_as_uint(__uint_as_float(s_w) * __uint_as_float(s_x)) : s_w << 8 | s_x;
+    auto bring_b = [&](int s, int buf) {
+        const char* const k = b0 + (long long)s * KROW;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) dma16s(k, from[PA + i], lds0 + buf * T::BUF + (BM / 8 + i * 8 + wave) * 1024);
     };
     auto phase_end = [&] {                                                    // (matrix instructions touch no memory: the scheduling barriers keep them in their phase)
         __builtin_amdgcn_sched_barrier(0);
@@ -539,29 +584,45 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
         __builtin_amdgcn_sched_barrier(0);
     };
 
+    auto pin = [&](const f32x4 (&row)[NT]) {                                  // the instructions that made these sums stay in front of what follows (they touch no memory:
+#pragma unroll
+        for (int j = 0; j < NT; ++j) asm volatile("" :: "v"(row[j]));         // the compiler would put them off, behind the waits)
+    };
+
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    bring(0);
-    landed(0);
+    bring_b(0, 0);
+    bring_a(0, 0);
+    if (steps > 1) { bring_b(1, 1); bring_a(1, 1); wait_all_but<PA + PB + PS>(); }
+    else wait_all_but<0>();
     phase_end();
     if (grp == 1) {
-        if (steps > 1) bring(1);
+        if (NBUF == 3 && steps > 2) { bring_b(2, 2); bring_a(2, 2); }
         phase_end();
     }
+    int buf = 0;                                                              // of step s; that of s + 2 (two buffers: the same)
     for (int s = 0; s < steps; ++s) {
-        const char* const xa = smem + (s & 1) * T::BUF;
+        const int buf2 = NBUF == 2 ? buf : buf == 0 ? 2 : buf - 1;
+        const char* const xa = smem + buf * T::BUF;
         const char* const wa = xa + BM * KROW;
+        const unsigned* const scales = reinterpret_cast<const unsigned*>(smem + NBUF * T::BUF + (s & 3) * T::SLOT);
+        const bool more = s + 2 < steps;
         Frag<IN, EXACT> w[NT];
+        unsigned sw = 0;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             // ---- L
+            if (grp == 0 && more && h == (NBUF == 3 ? 0 : H - 1)) {
+                bring_b(s + 2, buf2);
+                if (NBUF == 3) bring_a(s + 2, buf2);
+            }
             if (h == 0) {
-                if (grp == 0 && s + 1 < steps) bring(s + 1);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4));
+                if (PS) sw = scales[BM + wn / BLK];
             }
             Frag<IN, EXACT> x[XG];
             unsigned sv[XG];
@@ -569,29 +630,44 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             for (int i = 0; i < XG; ++i) {
                 const int row = wm + (h * XG + i) * 16 + r;
                 x[i].set(chunk(xa, row, q), chunk(xa, row, q + 4));
-                if (IN != IN_BF16) sv[i] = scales[(s & 1) * T::SCALES + (wn / BLK) * BM + row];
+                if (PS) sv[i] = scales[row];
             }
-            if (h == H - 1 && grp == 1 && s + 1 < steps) landed(s + 1);
+            if (h == H - 1 && grp == 1) {                                     // step s + 1 is there but for what was asked for after it
+                if (!more) wait_all_but<0>();
+                else if (NBUF == 3) wait_all_but<PA + PB + PS>();
+                else wait_all_but<PB>();
+            }
             phase_end();
             // ---- M
-            if (h == H - 1 && grp == 1 && s + 2 < steps) bring(s + 2);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < XG; ++i) {
                 Scale<IN, EXACT> sc;
-                if (IN != IN_BF16) sc.set(sv[i]);
+                if (PS) sc.set(sw, sv[i]);
                 mac_row<IN, EXACT, NT>(acc[h * XG + i], w, x[i], sc);
+                if (i == 0) {                                                 // (behind the first instructions: the pipe is busy while these are issued)
+                    pin(acc[h * XG]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (NBUF == 2) {
+                        if (h == 0 && grp == 1 && more) bring_b(s + 2, buf2);
+                        if (h == H - 1 && more) bring_a(s + 2, buf2);
+                    } else if (h == H - 1 && grp == 1 && s + 3 < steps) {
+                        bring_b(s + 3, buf);
+                        bring_a(s + 3, buf);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             __builtin_amdgcn_s_setprio(0);
-            if (h < H - 1) {                                                  // (the compiler would put them off to the end of the step)
 #pragma unroll
-                for (int i = 0; i < XG; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) asm volatile("" :: "v"(acc[h * XG + i][j]));
+            for (int i = 1; i < XG; ++i) pin(acc[h * XG + i]);
+            if (h == H - 1 && grp == 0) {
+                if (more) wait_all_but<PA + PB + PS>();
+                else wait_all_but<0>();
             }
-            if (h == H - 1 && grp == 0 && s + 1 < steps) landed(s + 1);
             phase_end();
         }
+        buf = buf == NBUF - 1 ? 0 : buf + 1;
     }
     if (grp == 0) phase_end();
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
@@ -608,9 +684,9 @@ template <int IN, int OUT>
 hipError_t launch_any(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + 127) / 128;
-    const long long tiles = row_tiles(p, 64) * p.tiles_n;
-    if (tiles > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    product_any_kernel<IN, OUT><<<(unsigned)tiles, 256, 0, st>>>(p);
+    const long long grid = (row_tiles(p, 64) * p.tiles_n + 7) / 8 * 8;
+    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    product_any_kernel<IN, OUT><<<(unsigned)grid, 256, 0, st>>>(p);
     return hipGetLastError();
 }
 
@@ -643,10 +719,10 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
     if (!aligned || p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
-    using T256 = Tile<2, 4, 8, 4>;
-    using T128W = Tile<2, 4, 4, 4>;
+    using T256 = Phased<2, 4, 8, 4, 2>;
+    using T128W = Phased<2, 4, 4, 4, 3>;
     using T128 = Tile<2, 2, 4, 4>;
-    const bool near = p.kbytes % KROW == 0 && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);
+    const bool near = p.kbytes % KROW == 0 && p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);
     if constexpr (IN == IN_BF16 || OUT != OUT_F32)
         if (near && row_tiles(p, 256) * ((p.n + 255) / 256) >= 256) return launch_phased<IN, OUT, T256>(p, st);
     if (near && row_tiles(p, 128) * ((p.n + 255) / 256) >= 256) return launch_phased<IN, OUT, T128W>(p, st);
