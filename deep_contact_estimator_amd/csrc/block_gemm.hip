@@ -11,7 +11,14 @@
 // The weights are the instruction's FIRST operand: a lane then holds four neighbouring columns of one row of y (one activation scale a lane, vector
 // stores).  Lane l: row l & 15 of either operand, chunks l >> 4 and (l >> 4) + 4.
 #include "block_ops.h"
+#include <cmath>
 
+#ifndef FORCE
+#define FORCE -1
+#endif
+#ifndef ROWS_T
+#define ROWS_T 64
+#endif
 namespace dce {
 
 namespace {
@@ -284,21 +291,13 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
     }
 }
 
-// ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave.  Both panels of a step
-//      come by LDS-DMA into one of two buffers while the matrix pipe works on the other; one barrier a step.
-__device__ __attribute__((aligned(16))) const char zero16[16] = {};
-
-// 64 lanes x 16 bytes from the lanes' addresses to LDS at `lds` (+ lane * 16)
-__device__ __forceinline__ void dma16(const char* from, unsigned lds)
-{
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(lds) : "memory");
-}
-// ... from `from` + the lanes' offsets
+// ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave.  A step's panels and scales
+//      come by LDS-DMA into a ring of NBUF buffers, NBUF - 1 steps ahead; one barrier a step.
+// 64 lanes x 16 bytes from `from` + the lanes' offsets to LDS at `lds` (+ lane * 16)
 __device__ __forceinline__ void dma16s(const char* from, unsigned at, unsigned lds)
 {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" :: "s"(from), "v"(at), "s"(lds) : "memory");
 }
-// ... 64 lanes x 4 bytes / 1 byte (widened to a word), a word a lane in LDS
 __device__ __forceinline__ void dma4s(const char* from, unsigned at, unsigned lds)
 {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %0" :: "s"(from), "v"(at), "s"(lds) : "memory");
@@ -309,13 +308,15 @@ __device__ __forceinline__ void dma1s(const char* from, unsigned at, unsigned ld
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p; }
 
-template <int WM_, int WN_, int MT_, int NT_> struct Tile {
-    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;              // waves along the rows / the columns; blocks of 16 a wave
+template <int N> __device__ __forceinline__ void wait_all_but() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+
+template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Ring {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;   // waves along the rows / the columns; blocks of 16 a wave
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr int BUF = (BM + BN) * KROW, PIECES = BUF / 1024 / WAVES;   // a piece: eight rows, one instruction
-    static constexpr int CB = BN / BLK, SCALES = BM * CB;
-    static constexpr int LDS = 2 * BUF + 2 * SCALES * 8;
-    static_assert(BUF % (1024 * WAVES) == 0 && BM % 8 == 0 && BN % BLK == 0 && SCALES <= THREADS, "tile");
+    static constexpr int PANELS = (BM + BN) * KROW, PIECES = PANELS / 1024 / WAVES;   // a piece: eight rows, one instruction
+    static constexpr int SLOT = ((BM + 63) / 64 * 64 + 64) * 4, BUF = PANELS + SLOT;  // the rows' scales, the columns': a word each
+    static constexpr int LDS = NBUF * BUF;
+    static_assert(PANELS % (1024 * WAVES) == 0 && BM % 8 == 0 && BN == BLK && LDS <= 160 * 1024 && (BM + 63) / 64 <= WAVES, "tile");
 };
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
@@ -393,8 +394,9 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
             __builtin_amdgcn_wave_barrier();
             constexpr int CH = ROW / 16;                                      // 16-byte pieces of a row
 #pragma unroll
-            for (int t = 0; t < CH * 16 / 64; ++t) {
+            for (int t = 0; t < (CH * 16 + 63) / 64; ++t) {
                 const int row = (t * 64 + lane) / CH, c = (t * 64 + lane) % CH;
+                if (row >= 16) break;
                 const i32x4 v = *reinterpret_cast<const i32x4*>(turn + row * PITCH + c * 16);
                 if (j0 + row < end) *reinterpret_cast<i32x4*>(y0 + (long long)(j0 + row) * p.y_row + c * 16) = v;
             }
@@ -410,58 +412,60 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
 }
 
 template <int IN, int OUT, class T>
-__global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs p)
+__global__ __launch_bounds__(T::THREADS) void product_ring_kernel(ProductArgs p)
 {
     constexpr bool EXACT = OUT == OUT_F32;
-    constexpr int BM = T::BM, BN = T::BN, MT = T::MT, NT = T::NT;
+    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, NBUF = T::NBUF, PS = IN != IN_BF16 ? 2 : 0;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    uint2* const scales = reinterpret_cast<uint2*>(smem + 2 * T::BUF);        // [2][column block][row]: the weights', x's
-    Place at;
-    if (!find_tile(p, BM, at)) return;
-    const int g = at.g, first = at.first, end = at.end, tn = at.tn;
-    const int n0 = tn * BN, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    Place place;
+    if (!find_tile(p, BM, place)) return;
+    const int g = place.g, first = place.first, end = place.end, n0 = place.tn * T::BN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
     const int wm = (wave / T::WN) * MT * 16, wn = (wave % T::WN) * NT * 16;
     const int steps = (p.kbytes + KROW - 1) / KROW;
 
-    const char* from[T::PIECES];
-    int col16[T::PIECES];
+    unsigned from[T::PIECES];                                                 // from the step's column of a, of the group's b
 #pragma unroll
     for (int i = 0; i < T::PIECES; ++i) {
-        const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3);
-        col16[i] = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
-        if (i * T::WAVES * 8 < BM) {                                          // (a piece lies in one panel: BM is a multiple of a round's rows)
-            const long long s = source_row(p, first + lr, end);
-            from[i] = p.a + (s < 0 ? 0 : s) * p.a_row + col16[i];             // rows without a source: any row, taken out at the end
-        } else {
-            const int c = n0 + lr - BM;
-            from[i] = p.b + g * p.b_group + (long long)(c < p.n ? c : p.n - 1) * p.b_row + col16[i];
-        }
+        const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3), col = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
+        unsigned row;
+        if ((i * T::WAVES + wave) * 8 < BM) { const long long s = source_row(p, first + lr, end); row = (unsigned)(s < 0 ? 0 : s) * (unsigned)p.a_row; }   // (no source: any row, taken out at the end)
+        else { const int c = n0 + lr - BM; row = (unsigned)(c < p.n ? c : p.n - 1) * (unsigned)p.b_row; }
+        asm volatile("" : "+v"(row));                                         // (a product and a sum of 32 bits: not the instruction whose result fills two registers)
+        from[i] = row + col;
     }
-    static_assert(BM % (T::WAVES * 8) == 0, "a round of pieces lies in one panel");
+    // the scales of 64 rows (several waves may bring the same ones) and of the column block (all waves)
+    constexpr int SZ = IN == IN_F8_F32 ? 4 : 1;
+    const int s_row = wave % ((BM + 63) / 64) * 64;
+    const char *ka = p.a, *kb = p.b + g * p.b_group, *sa = static_cast<const char*>(p.sa), *sb = nullptr;
+    unsigned sa_at = 0, none = 0;
+    if (PS) {
+        const long long s = s_row + lane < BM ? source_row(p, first + s_row + lane, end) : -1;
+        sa_at = (unsigned)(s < 0 ? 0 : s) * SZ;
+        sb = static_cast<const char*>(p.sb) + (g * p.sb_group + (long long)place.tn * p.sb_row) * SZ;
+        asm volatile("" : "+v"(none));
+    }
     const unsigned lds0 = lds_addr(smem);
+    int to = 0;                                                               // the buffer of the next step asked for
+    const int tail = p.kbytes % KROW;                                         // bytes of the last step, where K ends inside it
+    auto tail_col = [&](int i) { const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3); return ((lane & 7) ^ ((lr >> 1) & 7)) * 16; };
     auto bring = [&](int s) {
-        const bool last = (s + 1) * KROW > p.kbytes;                          // a step that K ends inside: chunks behind it come from a zero
+        const unsigned at = lds0 + to * T::BUF;
+        if (tail && s == steps - 1) {                                         // chunks behind the end: any that are there, made zeros below
 #pragma unroll
-        for (int i = 0; i < T::PIECES; ++i) {
-            const char* a = from[i];
-            if (last && s * KROW + col16[i] >= p.kbytes) a = zero16;
-            dma16(a, lds0 + (s & 1) * T::BUF + (i * T::WAVES + wave) * 1024);
-            from[i] += KROW;
+            for (int i = 0; i < T::PIECES; ++i) if (tail_col(i) >= tail) from[i] -= tail_col(i);
         }
-    };
-    // the scale of row `tid` % BM and column block tid / BM, a step ahead in a register
-    long long sa_at = 0, sb_at = 0;
-    if (IN != IN_BF16 && tid < T::SCALES) {
-        const long long s = source_row(p, first + tid % BM, end);
-        sa_at = s < 0 ? 0 : s;
-        const int u = (n0 + BLK * (tid / BM)) / BLK, last = (p.n - 1) / BLK;
-        sb_at = g * p.sb_group + (long long)(u < last ? u : last) * p.sb_row;
-    }
-    unsigned s_x = 0, s_w = 0;
-    auto bring_scale = [&](int s) {
-        if (IN == IN_BF16 || tid >= T::SCALES) return;
-        if (IN == IN_F8_F32) { s_x = static_cast<const unsigned*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned*>(p.sb)[sb_at + s]; }
-        else { s_x = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + sa_at]; s_w = static_cast<const unsigned char*>(p.sb)[sb_at + s]; }
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i) dma16s((i * T::WAVES + wave) * 8 < BM ? ka : kb, from[i], at + (i * T::WAVES + wave) * 1024);
+        ka += KROW;
+        kb += KROW;
+        if constexpr (PS != 0) {
+            if constexpr (SZ == 4) { dma4s(sa, sa_at, at + T::PANELS + s_row * 4); dma4s(sb, none, at + T::PANELS + T::SLOT - 256); }
+            else { dma1s(sa, sa_at, at + T::PANELS + s_row * 4); dma1s(sb, none, at + T::PANELS + T::SLOT - 256); }
+            sa += p.sa_block * SZ;
+            sb += SZ;
+        }
+        to = to == NBUF - 1 ? 0 : to + 1;
     };
 
     f32x4 acc[MT][NT];
@@ -469,27 +473,46 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_tile_kernel(ProductArgs
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    bring_scale(0);
-    bring(0);
+#pragma unroll
+    for (int s = 0; s < NBUF - 1; ++s) if (s < steps) bring(s);
+    int buf = 0;
     for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (IN != IN_BF16 && tid < T::SCALES)
-            scales[(s & 1) * T::SCALES + tid] = make_uint2(s_w, s_x);
-        __syncthreads();                                                      // the step's panels are there, the other buffer has been read
-        if (s + 1 < steps) { bring_scale(s + 1); bring(s + 1); }
-        const char* xa = smem + (s & 1) * T::BUF;
-        const char* wa = xa + BM * KROW;
+        // step s has landed; the NBUF - 2 after it may be on their way (fewer at the end: all of them are waited for)
+        if (s + NBUF - 2 < steps) wait_all_but<(NBUF - 2) * (T::PIECES + PS)>();
+        else wait_all_but<0>();
+        char* const xa = smem + buf * T::BUF;
+        if (tail && s == steps - 1) {
+#pragma unroll
+            for (int i = 0; i < T::PIECES; ++i)
+                if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(xa + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // ... for every wave, and step s - 1 has been read
+        const char* const wa = xa + BM * KROW;
+        const unsigned* const scales = reinterpret_cast<const unsigned*>(xa + T::PANELS);
+        i32x4 w0[NT], w1[NT], x0[MT], x1[MT];
+        unsigned sw = 0, sx[MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) { w0[j] = chunk(wa, wn + j * 16 + r, q); w1[j] = chunk(wa, wn + j * 16 + r, q + 4); }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) { x0[i] = chunk(xa, wm + i * 16 + r, q); x1[i] = chunk(xa, wm + i * 16 + r, q + 4); }
+        if (PS) {
+            sw = scales[T::SLOT / 4 - 64];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sx[i] = scales[wm + i * 16 + r];
+        }
+        if (s + NBUF - 1 < steps) bring(s + NBUF - 1);                        // (while the fragments are on their way)
         Frag<IN, EXACT> w[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4));
+        for (int j = 0; j < NT; ++j) w[j].set(w0[j], w1[j]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             Frag<IN, EXACT> x;
-            x.set(chunk(xa, wm + i * 16 + r, q), chunk(xa, wm + i * 16 + r, q + 4));
+            x.set(x0[i], x1[i]);
             Scale<IN, EXACT> sc;
-            if (IN != IN_BF16) { const uint2 v = scales[(s & 1) * T::SCALES + (wn / BLK) * BM + wm + i * 16 + r]; sc.set(v.x, v.y); }
+            if (PS) sc.set(sw, sx[i]);
             mac_row<IN, EXACT, NT>(acc[i], w, x, sc);
         }
+        buf = buf == NBUF - 1 ? 0 : buf + 1;
     }
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
@@ -515,13 +538,11 @@ template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
     static_assert(WM == 2 && WN == 4 && BN / BLK <= 64 && (NBUF == 2 || NBUF == 3), "two groups of four waves");
 };
 
-template <int N> __device__ __forceinline__ void wait_all_but() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
-
 template <int IN, int OUT, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductArgs p)
 {
     constexpr bool EXACT = OUT == OUT_F32;
-    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, XG = EXACT && IN != IN_BF16 ? 2 : 4, H = MT / XG;   // (e4m3 as fp16 takes twice the registers)
+    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, XG = 4, H = MT / XG;
     constexpr int PA = T::PA, PB = T::PB, PS = IN != IN_BF16, NBUF = T::NBUF;
     static_assert(MT % XG == 0 && (NBUF == 3 || H == 2), "phases");
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -673,6 +694,91 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
+// ---- the kernel for few rows a group: 16 MT rows x 16 columns a workgroup, K dealt out to its sixteen waves step by step, the waves' sums added in LDS in
+//      their order.  What it does is read the weights once: operands go straight into registers, U steps of them asked for before the first is used.
+//      Any alignment.
+template <int IN, int OUT, int MT, int U>
+__global__ __launch_bounds__(1024) void product_rows_kernel(ProductArgs p)
+{
+    constexpr bool EXACT = OUT == OUT_F32;
+    constexpr int WAVES = 16;
+    __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][MT][64];
+    Place place;
+    if (!find_tile(p, MT * 16, place)) return;
+    const int g = place.g, first = place.first, end = place.end, n0 = place.tn * 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int steps = (p.kbytes + KROW - 1) / KROW;
+    const int c = n0 + r;
+    const char* const w_row = p.b + g * p.b_group + (long long)(c < p.n ? c : p.n - 1) * p.b_row;
+    const char* x_row[MT];
+    long long src[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const long long s = source_row(p, first + i * 16 + r, end);
+        src[i] = s < 0 ? 0 : s;                                               // rows without a source: any row, taken out at the end
+        x_row[i] = p.a + src[i] * p.a_row;
+    }
+    const long long sb0 = g * p.sb_group + (long long)(n0 / BLK) * p.sb_row;
+    f32x4 acc[MT][1];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
+        i32x4 w[U][2], x[U][MT][2];
+        unsigned sw[U], sx[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = s0 + u * WAVES;
+            if (s < steps) {
+                const int at = s * KROW + q * 16;
+                if ((s + 1) * KROW <= p.kbytes) {
+                    w[u][0] = load16(w_row + at); w[u][1] = load16(w_row + at + 64);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) { x[u][i][0] = load16(x_row[i] + at); x[u][i][1] = load16(x_row[i] + at + 64); }
+                } else {
+                    w[u][0] = load16_tail(w_row, at, p.kbytes); w[u][1] = load16_tail(w_row, at + 64, p.kbytes);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) { x[u][i][0] = load16_tail(x_row[i], at, p.kbytes); x[u][i][1] = load16_tail(x_row[i], at + 64, p.kbytes); }
+                }
+                if (IN == IN_F8_F32) {
+                    sw[u] = static_cast<const unsigned*>(p.sb)[sb0 + s];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) sx[u][i] = static_cast<const unsigned*>(p.sa)[s * p.sa_block + src[i]];
+                } else if (IN == IN_F8_E8) {
+                    sw[u] = static_cast<const unsigned char*>(p.sb)[sb0 + s];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) sx[u][i] = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + src[i]];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u * WAVES < steps) {
+                Frag<IN, EXACT> wf[1], xf;
+                wf[0].set(w[u][0], w[u][1]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    xf.set(x[u][i][0], x[u][i][1]);
+                    Scale<IN, EXACT> sc;
+                    if (IN != IN_BF16) sc.set(sw[u], sx[u][i]);
+                    mac_row<IN, EXACT, 1>(acc[i], wf, xf, sc);
+                }
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i][0];
+    __syncthreads();
+    if (threadIdx.x >= MT * 64) return;
+    const int j = first + wave * 16 + r;                                      // (waves 0 .. MT - 1: a row tile each)
+    f32x4 y = part[0][wave][lane];
+#pragma unroll
+    for (int u = 1; u < WAVES; ++u) y += part[u][wave][lane];
+    if (j >= end) return;
+    if (p.index && source_row(p, j, end) < 0) y = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int col = n0 + q * 4;
+    y = finish(p, y, p.bias ? p.bias + g * p.bias_group : nullptr, col);
+    if (col < p.n) store4<OUT>(p, j, col, y, wide_stores(p, OUT == OUT_F32 ? 16 : 8));
+}
+
 namespace {
 
 long long row_tiles(const ProductArgs& p, int bm)                             // at most: a group of rows ends inside a tile
@@ -691,14 +797,14 @@ hipError_t launch_any(ProductArgs p, hipStream_t st)
 }
 
 template <int IN, int OUT, class T>
-hipError_t launch_tile(ProductArgs p, hipStream_t st)
+hipError_t launch_ring(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(product_tile_kernel<IN, OUT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(product_ring_kernel<IN, OUT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
     if (once != hipSuccess) return once;
-    product_tile_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
+    product_ring_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
 
@@ -714,19 +820,54 @@ hipError_t launch_phased(ProductArgs p, hipStream_t st)
     return hipGetLastError();
 }
 
+template <int IN, int OUT, int MT, int U>
+hipError_t launch_rows(ProductArgs p, hipStream_t st)
+{
+    p.tiles_n = (p.n + 15) / 16;
+    const long long grid = (row_tiles(p, MT * 16) * p.tiles_n + 7) / 8 * 8;
+    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    product_rows_kernel<IN, OUT, MT, U><<<(unsigned)grid, 1024, 0, st>>>(p);
+    return hipGetLastError();
+}
+
 template <int IN, int OUT>
 hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
+    const int mean = (p.m + p.groups - 1) / p.groups;                         // rows a group
+    if constexpr (OUT != OUT_E4M3)
+        if (p.a_rows > 0 && p.kbytes > 0 && mean <= ROWS_T) {
+            if (mean <= 16) return launch_rows<IN, OUT, 1, 3>(p, st);
+            return launch_rows<IN, OUT, 2, 2>(p, st);
+        }
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
-    if (!aligned || p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
-    using T256 = Phased<2, 4, 8, 4, 2>;
-    using T128W = Phased<2, 4, 4, 4, 3>;
-    using T128 = Tile<2, 2, 4, 4>;
-    const bool near = p.kbytes % KROW == 0 && p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);
-    if constexpr (IN == IN_BF16 || OUT != OUT_F32)
-        if (near && row_tiles(p, 256) * ((p.n + 255) / 256) >= 256) return launch_phased<IN, OUT, T256>(p, st);
-    if (near && row_tiles(p, 128) * ((p.n + 255) / 256) >= 256) return launch_phased<IN, OUT, T128W>(p, st);
-    return launch_tile<IN, OUT, T128>(p, st);
+    const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // (32-bit offsets)
+    if (!aligned || !near || p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
+    const bool whole = p.kbytes % KROW == 0;
+    // what a row of tiles' steps cost: rounds of a tile on every CU, times its step
+    const double rows = p.offsets ? p.m + 0.5 : p.m;
+    auto cost = [&](int bm, int bn, double step) {
+        const double tiles = (p.offsets ? (double)p.m / bm + 0.5 * (p.groups < p.m ? p.groups : p.m) : (double)((p.m + bm - 1) / bm)) * ((p.n + bn - 1) / bn);
+        return ceil(tiles / 256.0) * step;
+    };
+    (void)rows;
+    constexpr bool F16 = OUT == OUT_F32 && IN != IN_BF16;                     // e4m3 as fp16
+    const double c32 = cost(32, 128, 0.30), c64 = cost(64, 128, 0.36), c128 = cost(128, 128, 0.5);
+    const double w128 = whole ? cost(128, 256, F16 ? 1.3 : 0.9) : 1e30, w256 = whole && !F16 ? cost(256, 256, 1.5) : 1e30;
+    double best = c32; int pick = FORCE;
+    if (pick < 0) {
+        pick = 0;
+        if (c64 <= best) { best = c64; pick = 1; }
+        if (c128 <= best) { best = c128; pick = 2; }
+        if (w128 <= best) { best = w128; pick = 3; }
+        if (w256 <= best) { best = w256; pick = 4; }
+    }
+    if (pick >= 3 && !whole) pick = 2;
+    if (F16 && pick == 4) pick = 3;
+    if constexpr (!F16) if (pick == 4) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
+    if (pick == 3) return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
+    if (pick == 2) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);
+    if (pick == 1) return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 5>>(p, st);
+    return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 6>>(p, st);
 }
 
 template <int IN>
