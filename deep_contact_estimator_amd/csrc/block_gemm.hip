@@ -207,7 +207,7 @@ __device__ __forceinline__ bool wide_stores(const ProductArgs& p, int bytes)
 
 // ---- the kernel for every case: 64 rows x 128 columns a workgroup, sixteen rows a wave; operands through registers into LDS, from any alignment
 template <int IN, int OUT>
-__global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
+__global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
 {
     constexpr int BM = 64, BN = 128, CH = (BM + BN) * 8 / 256;               // 16-byte chunks a thread brings each step
     constexpr bool EXACT = OUT == OUT_F32;
@@ -292,7 +292,8 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs p)
 }
 
 // ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave.  A step's panels and scales
-//      come by LDS-DMA into a ring of NBUF buffers, NBUF - 1 steps ahead; one barrier a step.
+//      come by LDS-DMA into a ring of NBUF buffers, NBUF - 1 steps ahead, fragments from there into registers a step ahead of their instructions; one
+//      barrier a step.
 // 64 lanes x 16 bytes from `from` + the lanes' offsets to LDS at `lds` (+ lane * 16)
 __device__ __forceinline__ void dma16s(const char* from, unsigned at, unsigned lds)
 {
@@ -412,7 +413,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
 }
 
 template <int IN, int OUT, class T>
-__global__ __launch_bounds__(T::THREADS) void product_ring_kernel(ProductArgs p)
+__global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs p)
 {
     constexpr bool EXACT = OUT == OUT_F32;
     constexpr int BM = T::BM, MT = T::MT, NT = T::NT, NBUF = T::NBUF, PS = IN != IN_BF16 ? 2 : 0;
@@ -449,14 +450,17 @@ __global__ __launch_bounds__(T::THREADS) void product_ring_kernel(ProductArgs p)
     int to = 0;                                                               // the buffer of the next step asked for
     const int tail = p.kbytes % KROW;                                         // bytes of the last step, where K ends inside it
     auto tail_col = [&](int i) { const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3); return ((lane & 7) ^ ((lr >> 1) & 7)) * 16; };
-    auto bring = [&](int s) {
+    // pieces lo .. hi - 1 of step s (the last ones: its scales)
+    constexpr int ALL = T::PIECES + PS;
+    auto bring = [&](int s, int lo, int hi) {
         const unsigned at = lds0 + to * T::BUF;
-        if (tail && s == steps - 1) {                                         // chunks behind the end: any that are there, made zeros below
+        if (lo == 0 && tail && s == steps - 1) {                                         // chunks behind the end: any that are there, made zeros below
 #pragma unroll
             for (int i = 0; i < T::PIECES; ++i) if (tail_col(i) >= tail) from[i] -= tail_col(i);
         }
 #pragma unroll
-        for (int i = 0; i < T::PIECES; ++i) dma16s((i * T::WAVES + wave) * 8 < BM ? ka : kb, from[i], at + (i * T::WAVES + wave) * 1024);
+        for (int i = 0; i < T::PIECES; ++i) if (i >= lo && i < hi) dma16s((i * T::WAVES + wave) * 8 < BM ? ka : kb, from[i], at + (i * T::WAVES + wave) * 1024);
+        if (hi < ALL) return;
         ka += KROW;
         kb += KROW;
         if constexpr (PS != 0) {
@@ -474,45 +478,73 @@ __global__ __launch_bounds__(T::THREADS) void product_ring_kernel(ProductArgs p)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < NBUF - 1; ++s) if (s < steps) bring(s);
+    for (int s = 0; s < NBUF; ++s) if (s < steps) bring(s, 0, ALL);
     int buf = 0;
-    for (int s = 0; s < steps; ++s) {
-        // step s has landed; the NBUF - 2 after it may be on their way (fewer at the end: all of them are waited for)
+    struct Step { i32x4 w0[NT], w1[NT], x0[MT], x1[MT]; unsigned sw, sx[MT]; } even, odd;
+    // step s is there, for every wave, and the fragments of step s - 1 have been read (so its buffer is free); the NBUF - 2 steps behind it may be on
+    // their way (fewer at the end: all of them are waited for)
+    auto arrive = [&](int s) {
         if (s + NBUF - 2 < steps) wait_all_but<(NBUF - 2) * (T::PIECES + PS)>();
         else wait_all_but<0>();
-        char* const xa = smem + buf * T::BUF;
         if (tail && s == steps - 1) {
 #pragma unroll
             for (int i = 0; i < T::PIECES; ++i)
-                if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(xa + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
+                if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(smem + buf * T::BUF + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
         }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // ... for every wave, and step s - 1 has been read
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto read = [&](Step& f) {
+        const char* const xa = smem + buf * T::BUF;
         const char* const wa = xa + BM * KROW;
         const unsigned* const scales = reinterpret_cast<const unsigned*>(xa + T::PANELS);
-        i32x4 w0[NT], w1[NT], x0[MT], x1[MT];
-        unsigned sw = 0, sx[MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) { w0[j] = chunk(wa, wn + j * 16 + r, q); w1[j] = chunk(wa, wn + j * 16 + r, q + 4); }
+        for (int j = 0; j < NT; ++j) { f.w0[j] = chunk(wa, wn + j * 16 + r, q); f.w1[j] = chunk(wa, wn + j * 16 + r, q + 4); }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) { x0[i] = chunk(xa, wm + i * 16 + r, q); x1[i] = chunk(xa, wm + i * 16 + r, q + 4); }
+        for (int i = 0; i < MT; ++i) { f.x0[i] = chunk(xa, wm + i * 16 + r, q); f.x1[i] = chunk(xa, wm + i * 16 + r, q + 4); }
         if (PS) {
-            sw = scales[T::SLOT / 4 - 64];
+            f.sw = scales[T::SLOT / 4 - 64];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) sx[i] = scales[wm + i * 16 + r];
+            for (int i = 0; i < MT; ++i) f.sx[i] = scales[wm + i * 16 + r];
         }
-        if (s + NBUF - 1 < steps) bring(s + NBUF - 1);                        // (while the fragments are on their way)
+        buf = buf == NBUF - 1 ? 0 : buf + 1;
+    };
+    auto step = [&](int s, const Step& f, Step& next) {
+        if (s + 1 < steps) {
+            arrive(s + 1);
+            read(next);
+        }
         Frag<IN, EXACT> w[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j].set(w0[j], w1[j]);
+        for (int j = 0; j < NT; ++j) w[j].set(f.w0[j], f.w1[j]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             Frag<IN, EXACT> x;
-            x.set(x0[i], x1[i]);
+            x.set(f.x0[i], f.x1[i]);
             Scale<IN, EXACT> sc;
-            if (PS) sc.set(sw, sx[i]);
+            if (PS) sc.set(f.sw, f.sx[i]);
             mac_row<IN, EXACT, NT>(acc[i], w, x, sc);
+            if (s + NBUF < steps) {                                           // requests between the instructions, some behind each row: the pipe is busy while they are issued
+#pragma unroll
+                for (int j = 0; j < NT; ++j) asm volatile("" :: "v"(acc[i][j]));
+                __builtin_amdgcn_sched_barrier(0);
+                bring(s + NBUF, i * ALL / MT, (i + 1) * ALL / MT);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        buf = buf == NBUF - 1 ? 0 : buf + 1;
+    };
+    // (step 0 alone: NBUF steps are under way, and one fewer behind it than `arrive` counts on)
+    if (NBUF - 1 < steps) wait_all_but<(NBUF - 1) * (T::PIECES + PS)>();
+    else wait_all_but<0>();
+    if (tail && steps == 1) {
+#pragma unroll
+        for (int i = 0; i < T::PIECES; ++i)
+            if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(smem + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    read(even);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, even, odd);
+        if (s + 1 < steps) step(s + 1, odd, even);
     }
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
@@ -527,8 +559,9 @@ __global__ __launch_bounds__(T::THREADS) void product_ring_kernel(ProductArgs p)
 //
 // 64 KB a step and CU are 1 us of what L2 gives to all CUs at once (measured, 17 TB/s) and another half before the first of them is there, against 0.9 us
 // of matrix instructions: panels have to be asked for more than a step ahead.  256 x 256 tiles leave room for two buffers, so each part of a panel is
-// asked for as soon as its buffer has been read for the last time: step s + 2's weights at phase 4s + 2, group 0's rows at 4s + 3, group 1's at
-// 4s + 4.  128 x 256 tiles have three buffers: step s + 2 at phase 2H s.  Scales come the same way, a word a row.
+// asked for once its buffer has been read for the last time, a quarter of a step's requests (they take the CU 1150 cycles in all) in every phase: of step
+// s + 2, group 1's half of the weights at phase 4s + 2, group 0's rows at 4s + 3, group 1's at 4s + 4, group 0's half of the weights at 4s + 5.  128 x 256 tiles have three buffers: step s + 2 at phase 2H s + 1, by group 1 at 2H s.  All of it between matrix
+// instructions.  Scales come the same way, a word a row.
 template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
     static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
@@ -584,21 +617,20 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
         s_at = (unsigned)((u < last ? u : last) - n0 / BLK) * (unsigned)(p.sb_row * SZ);
         s_to = BM * 4;
     }
-    auto bring_a = [&](int s, int buf) {
-        const char* const k = p.a + (long long)s * KROW;
-        if constexpr (PS) {
-            const unsigned to = lds0 + NBUF * T::BUF + (s & 3) * T::SLOT + s_to;
-            if constexpr (SZ == 4) dma4s(s_from + s * s_step, s_at, to);
-            else dma1s(s_from + s * s_step, s_at, to);
+    // pieces lo .. hi - 1 of a step: the weights' (PB), the scales (PS), the group's rows (PA)
+    auto bring = [&](int s, int buf, int lo, int hi) {
+#pragma unroll
+        for (int t = 0; t < PB + PS + PA; ++t) {
+            if (t < lo || t >= hi) continue;
+            if (t < PB) dma16s(b0 + (long long)s * KROW, from[PA + t], lds0 + buf * T::BUF + (BM / 8 + t * 8 + wave) * 1024);
+            else if (t < PB + PS) {
+                const unsigned to = lds0 + NBUF * T::BUF + (s & 3) * T::SLOT + s_to;
+                if constexpr (SZ == 4) dma4s(s_from + s * s_step, s_at, to);
+                else dma1s(s_from + s * s_step, s_at, to);
+            } else dma16s(p.a + (long long)s * KROW, from[t - PB - PS], lds0 + buf * T::BUF + (grp * (BM / 16) + (t - PB - PS) * 4 + w4) * 1024);
         }
-#pragma unroll
-        for (int i = 0; i < PA; ++i) dma16s(k, from[i], lds0 + buf * T::BUF + (grp * (BM / 16) + i * 4 + w4) * 1024);
     };
-    auto bring_b = [&](int s, int buf) {
-        const char* const k = b0 + (long long)s * KROW;
-#pragma unroll
-        for (int i = 0; i < PB; ++i) dma16s(k, from[PA + i], lds0 + buf * T::BUF + (BM / 8 + i * 8 + wave) * 1024);
-    };
+    constexpr int ALL = PB + PS + PA;
     auto phase_end = [&] {                                                    // (matrix instructions touch no memory: the scheduling barriers keep them in their phase)
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -615,13 +647,12 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    bring_b(0, 0);
-    bring_a(0, 0);
-    if (steps > 1) { bring_b(1, 1); bring_a(1, 1); wait_all_but<PA + PB + PS>(); }
+    bring(0, 0, 0, ALL);
+    if (steps > 1) { bring(1, 1, 0, ALL); wait_all_but<ALL>(); }
     else wait_all_but<0>();
     phase_end();
     if (grp == 1) {
-        if (NBUF == 3 && steps > 2) { bring_b(2, 2); bring_a(2, 2); }
+        if (NBUF == 3 && steps > 2) bring(2, 2, 0, ALL);
         phase_end();
     }
     int buf = 0;                                                              // of step s; that of s + 2 (two buffers: the same)
@@ -636,10 +667,6 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             // ---- L
-            if (grp == 0 && more && h == (NBUF == 3 ? 0 : H - 1)) {
-                bring_b(s + 2, buf2);
-                if (NBUF == 3) bring_a(s + 2, buf2);
-            }
             if (h == 0) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4));
@@ -655,7 +682,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             }
             if (h == H - 1 && grp == 1) {                                     // step s + 1 is there but for what was asked for after it
                 if (!more) wait_all_but<0>();
-                else if (NBUF == 3) wait_all_but<PA + PB + PS>();
+                else if (NBUF == 3) wait_all_but<ALL>();
                 else wait_all_but<PB>();
             }
             phase_end();
@@ -666,25 +693,33 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
                 Scale<IN, EXACT> sc;
                 if (PS) sc.set(sw, sv[i]);
                 mac_row<IN, EXACT, NT>(acc[h * XG + i], w, x[i], sc);
-                if (i == 0) {                                                 // (behind the first instructions: the pipe is busy while these are issued)
-                    pin(acc[h * XG]);
+                // requests between the instructions, a few behind each row: the pipe is busy while they are issued
+                int next = s + 2;
+                bool ask;
+                if constexpr (NBUF == 2) {
+                    if (grp == 0) { next = h == 0 ? s + 1 : s + 2; ask = next < steps && (h > 0 || s > 0); }
+                    else ask = more;
+                } else {
+                    next = s + 2 + grp;
+                    ask = next < steps && h == (grp == 0 ? 0 : H - 1);
+                }
+                if (ask && i < XG - 1) {
+                    const int to = NBUF == 2 ? next & 1 : grp == 0 ? buf2 : buf;
+                    pin(acc[h * XG + i]);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (NBUF == 2) {
-                        if (h == 0 && grp == 1 && more) bring_b(s + 2, buf2);
-                        if (h == H - 1 && more) bring_a(s + 2, buf2);
-                    } else if (h == H - 1 && grp == 1 && s + 3 < steps) {
-                        bring_b(s + 3, buf);
-                        bring_a(s + 3, buf);
-                    }
+                    if (NBUF == 3) bring(next, to, i * ALL / (XG - 1), (i + 1) * ALL / (XG - 1));
+                    else if (h == 0) bring(next, to, i * PB / (XG - 1), (i + 1) * PB / (XG - 1));
+                    else bring(next, to, PB + i * (PS + PA) / (XG - 1), PB + (i + 1) * (PS + PA) / (XG - 1));
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-            for (int i = 1; i < XG; ++i) pin(acc[h * XG + i]);
+            for (int i = 0; i < XG; ++i) pin(acc[h * XG + i]);
             if (h == H - 1 && grp == 0) {
-                if (more) wait_all_but<PA + PB + PS>();
-                else wait_all_but<0>();
+                if (!more) wait_all_but<0>();
+                else if (NBUF == 3) wait_all_but<ALL>();
+                else wait_all_but<PA + PS>();
             }
             phase_end();
         }
@@ -851,7 +886,7 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     };
     (void)rows;
     constexpr bool F16 = OUT == OUT_F32 && IN != IN_BF16;                     // e4m3 as fp16
-    const double c32 = cost(32, 128, 0.30), c64 = cost(64, 128, 0.36), c128 = cost(128, 128, 0.5);
+    const double c32 = cost(32, 128, 0.30), c64 = cost(64, 128, 0.36), c128 = F16 ? 1e30 : cost(128, 128, 0.5);
     const double w128 = whole ? cost(128, 256, F16 ? 1.3 : 0.9) : 1e30, w256 = whole && !F16 ? cost(256, 256, 1.5) : 1e30;
     double best = c32; int pick = FORCE;
     if (pick < 0) {
@@ -863,9 +898,10 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     }
     if (pick >= 3 && !whole) pick = 2;
     if (F16 && pick == 4) pick = 3;
+    if (F16 && pick == 2) pick = 1;
     if constexpr (!F16) if (pick == 4) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
     if (pick == 3) return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
-    if (pick == 2) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);
+    if constexpr (!F16) if (pick == 2) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);
     if (pick == 1) return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 5>>(p, st);
     return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 6>>(p, st);
 }
