@@ -205,92 +205,6 @@ __device__ __forceinline__ bool wide_stores(const ProductArgs& p, int bytes)
 
 }  // namespace
 
-// ---- the kernel for every case: 64 rows x 128 columns a workgroup, sixteen rows a wave; operands through registers into LDS, from any alignment
-template <int IN, int OUT>
-__global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
-{
-    constexpr int BM = 64, BN = 128, CH = (BM + BN) * 8 / 256;               // 16-byte chunks a thread brings each step
-    constexpr bool EXACT = OUT == OUT_F32;
-    __shared__ __attribute__((aligned(16))) char lds[(BM + BN) * KROW];
-    Place at;
-    if (!find_tile(p, BM, at)) return;
-    const int g = at.g, first = at.first, end = at.end, tn = at.tn;
-    const int n0 = tn * BN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    const int steps = (p.kbytes + KROW - 1) / KROW;
-
-    const char* row[CH];                                                      // null: a row of zeros
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        const int lr = (int)(threadIdx.x >> 3) + 32 * i;
-        row[i] = nullptr;
-        if (lr < BM) { const long long s = source_row(p, first + lr, end); if (s >= 0) row[i] = p.a + s * p.a_row; }
-        else if (n0 + lr - BM < p.n) row[i] = p.b + g * p.b_group + (long long)(n0 + lr - BM) * p.b_row;
-    }
-    const int c8 = threadIdx.x & 7;
-    auto fetch = [&](int s, i32x4 (&v)[CH]) {
-#pragma unroll
-        for (int i = 0; i < CH; ++i) v[i] = row[i] ? load16_tail(row[i], s * KROW + c8 * 16, p.kbytes) : i32x4{0, 0, 0, 0};
-    };
-    const long long mine = source_row(p, first + wave * 16 + r, end);         // the row whose scales this lane applies
-    const long long sb0 = g * p.sb_group + (long long)tn * p.sb_row;
-
-    f32x4 acc[2][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i >> 2][i & 3] = f32x4{0.f, 0.f, 0.f, 0.f};
-    i32x4 next[CH];
-    if (steps) fetch(0, next);
-    for (int s = 0; s < steps; ++s) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int lr = (int)(threadIdx.x >> 3) + 32 * i;
-            *reinterpret_cast<i32x4*>(lds + slot_of(lr, c8)) = next[i];
-        }
-        __syncthreads();
-        Scale<IN, EXACT> sc;
-        if constexpr (IN == IN_F8_F32) sc.set(static_cast<const unsigned*>(p.sb)[sb0 + s], mine >= 0 ? static_cast<const unsigned*>(p.sa)[s * p.sa_block + mine] : 0x3f800000u);
-        if constexpr (IN == IN_F8_E8) sc.set(static_cast<const unsigned char*>(p.sb)[sb0 + s], mine >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine] : 127u);
-        if (s + 1 < steps) fetch(s + 1, next);
-        const int xr = wave * 16 + r;
-        Frag<IN, EXACT> x;
-        x.set(chunk(lds, xr, q), chunk(lds, xr, q + 4));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            Frag<IN, EXACT> w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { const int wr = BM + (h * 4 + j) * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4)); }
-            mac_row<IN, EXACT, 4>(acc[h], w, x, sc);
-        }
-    }
-    const int j = first + wave * 16 + r;
-    const float* bias = p.bias ? p.bias + g * p.bias_group : nullptr;
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) acc[nt >> 2][nt & 3] = finish(p, acc[nt >> 2][nt & 3], bias, n0 + nt * 16 + q * 4);
-    float inv = 1.f;
-    if constexpr (OUT == OUT_E4M3) {
-        float most = 0.f;                                                     // (columns from n on hold bias-free zeros of zero rows)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) most = fmaxf(most, finite_abs(acc[nt >> 2][nt & 3][i]));
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const int e = block_exponent(most);
-        inv = two_to(-e);
-        if (q == 0 && j < end) {
-            if (IN == IN_F8_E8) static_cast<unsigned char*>(p.ys)[tn * p.ys_block + j] = (unsigned char)(e + 127);
-            else static_cast<float*>(p.ys)[tn * p.ys_block + j] = two_to(e);
-        }
-    }
-    if (j >= end) return;
-    const bool wide = wide_stores(p, OUT == OUT_F32 ? 16 : OUT == OUT_BF16 ? 8 : 4);
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) {
-        const int c = n0 + nt * 16 + q * 4;
-        if (c < p.n) store4<OUT>(p, j, c, acc[nt >> 2][nt & 3] * inv, wide);
-    }
-}
-
 // ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave.  A step's panels and scales
 //      come by LDS-DMA into a ring of NBUF buffers, NBUF - 1 steps ahead, fragments from there into registers a step ahead of their instructions; one
 //      barrier a step.
@@ -550,6 +464,92 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
+// ---- the kernel for every case: 32 rows x 128 columns a workgroup, 32 columns a wave; operands through registers into LDS, from any alignment, two
+//      steps ahead in registers; two LDS buffers, one barrier a step
+struct AnyTile {
+    static constexpr int WM = 1, WN = 4, MT = 2, NT = 2, BM = 32, BN = 128, WAVES = 4, LDS = 2 * (BM + BN) * KROW;
+};
+
+template <int IN, int OUT>
+__global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
+{
+    constexpr int BM = 32, BN = 128, CH = (BM + BN) * 8 / 256;               // 16-byte chunks a thread brings each step
+    constexpr bool EXACT = OUT == OUT_F32;
+    using T = AnyTile;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    Place at;
+    if (!find_tile(p, BM, at)) return;
+    const int g = at.g, first = at.first, end = at.end, tn = at.tn;
+    const int n0 = tn * BN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int steps = (p.kbytes + KROW - 1) / KROW;
+
+    const char* row[CH];                                                      // null: a row of zeros
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int lr = (int)(threadIdx.x >> 3) + 32 * i;
+        row[i] = nullptr;
+        if (lr < BM) { const long long s = source_row(p, first + lr, end); if (s >= 0) row[i] = p.a + s * p.a_row; }
+        else if (n0 + lr - BM < p.n) row[i] = p.b + g * p.b_group + (long long)(n0 + lr - BM) * p.b_row;
+    }
+    const int c8 = threadIdx.x & 7;
+    long long mine[2];                                                        // the rows whose scales this lane applies
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mine[i] = source_row(p, first + i * 16 + r, end);
+    const long long sb0 = g * p.sb_group + (long long)tn * p.sb_row;
+    struct Step { i32x4 v[CH]; unsigned sw, sx[2]; } even, odd;
+    auto fetch = [&](int s, Step& f) {
+        if ((s + 1) * KROW <= p.kbytes) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) f.v[i] = row[i] ? load16(row[i] + s * KROW + c8 * 16) : i32x4{0, 0, 0, 0};
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) f.v[i] = row[i] ? load16_tail(row[i], s * KROW + c8 * 16, p.kbytes) : i32x4{0, 0, 0, 0};
+        }
+        if constexpr (IN == IN_F8_F32) {
+            f.sw = static_cast<const unsigned*>(p.sb)[sb0 + s];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) f.sx[i] = mine[i] >= 0 ? static_cast<const unsigned*>(p.sa)[s * p.sa_block + mine[i]] : 0x3f800000u;
+        }
+        if constexpr (IN == IN_F8_E8) {
+            f.sw = static_cast<const unsigned char*>(p.sb)[sb0 + s];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) f.sx[i] = mine[i] >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine[i]] : 127u;
+        }
+    };
+
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto step = [&](int s, Step& f) {
+        char* const lds = smem + (s & 1) * (BM + BN) * KROW;                  // (last read two steps ago: a barrier lies between)
+#pragma unroll
+        for (int i = 0; i < CH; ++i) *reinterpret_cast<i32x4*>(lds + slot_of((int)(threadIdx.x >> 3) + 32 * i, c8)) = f.v[i];
+        const unsigned sw = f.sw, sx[2] = {f.sx[0], f.sx[1]};
+        if (s + 2 < steps) fetch(s + 2, f);
+        __syncthreads();
+        Frag<IN, EXACT> w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { const int wr = BM + wave * 32 + j * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4)); }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            Frag<IN, EXACT> x;
+            x.set(chunk(lds, i * 16 + r, q), chunk(lds, i * 16 + r, q + 4));
+            Scale<IN, EXACT> sc;
+            if (IN != IN_BF16) sc.set(sw, sx[i]);
+            mac_row<IN, EXACT, 2>(acc[i], w, x, sc);
+        }
+    };
+    even.sw = odd.sw = even.sx[0] = even.sx[1] = odd.sx[0] = odd.sx[1] = 0;
+    if (steps > 0) fetch(0, even);
+    if (steps > 1) fetch(1, odd);
+    for (int s = 0; s < steps; s += 2) {
+        step(s, even);
+        if (s + 1 < steps) step(s + 1, odd);
+    }
+    __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
+    store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
+}
+
 // ---- the kernel for chip-filling products (K a multiple of 128 bytes, operands within 4 GB): eight waves in two groups that are a phase apart.
 //
 // Waves w and w + 4 share a SIMD.  While one group's phase is its matrix instructions, the other group's is reads of fragments from LDS and waits: the
@@ -575,7 +575,7 @@ template <int IN, int OUT, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductArgs p)
 {
     constexpr bool EXACT = OUT == OUT_F32;
-    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, XG = 4, H = MT / XG;
+    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, XG = MT % 4 == 0 ? 4 : 3, H = MT / XG;
     constexpr int PA = T::PA, PB = T::PB, PS = IN != IN_BF16, NBUF = T::NBUF;
     static_assert(MT % XG == 0 && (NBUF == 3 || H == 2), "phases");
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -824,10 +824,10 @@ long long row_tiles(const ProductArgs& p, int bm)                             //
 template <int IN, int OUT>
 hipError_t launch_any(ProductArgs p, hipStream_t st)
 {
-    p.tiles_n = (p.n + 127) / 128;
-    const long long grid = (row_tiles(p, 64) * p.tiles_n + 7) / 8 * 8;
+    p.tiles_n = (p.n + AnyTile::BN - 1) / AnyTile::BN;
+    const long long grid = (row_tiles(p, AnyTile::BM) * p.tiles_n + 7) / 8 * 8;
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    product_any_kernel<IN, OUT><<<(unsigned)grid, 256, 0, st>>>(p);
+    product_any_kernel<IN, OUT><<<(unsigned)grid, 256, AnyTile::LDS, st>>>(p);
     return hipGetLastError();
 }
 
@@ -897,8 +897,9 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
         if (w256 <= best) { best = w256; pick = 4; }
     }
     if (pick >= 3 && !whole) pick = 2;
-    if (F16 && pick == 4) pick = 3;
+    if (F16 && pick >= 4) pick = 3;
     if (F16 && pick == 2) pick = 1;
+    if constexpr (!F16) if (pick == 5) return launch_phased<IN, OUT, Phased<2, 4, 6, 4, 2>>(p, st);
     if constexpr (!F16) if (pick == 4) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
     if (pick == 3) return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
     if constexpr (!F16) if (pick == 2) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);

@@ -11,13 +11,16 @@ constexpr int64_t ROWS_MAX = 1ll << 30, DIM_MAX = 1ll << 24;
 
 bool off(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
+int device_count()
+{
+    static const int n = [] { int c = 0; return hipGetDeviceCount(&c) == hipSuccess ? c : 0; }();
+    return n;
+}
+
 #define OP_DEVICE(id)                                                                                                        \
-    int ndev_ = 0;                                                                                                           \
-    { const hipError_t e_ = hipGetDeviceCount(&ndev_);                                                                       \
-      if (e_ != hipSuccess || ndev_ <= 0)                                                                                    \
-          return fail(nullptr, DCE_ERR_HIP, "no HIP device available (%s): the HIP path is mandatory, there is no CPU fallback", \
-                      e_ == hipSuccess ? "device count 0" : hipGetErrorString(e_)); }                                        \
-    if ((id) < 0 || (id) >= ndev_) return fail(nullptr, DCE_ERR_ARG, "device %d out of range (%d devices)", (id), ndev_);    \
+    if (device_count() <= 0)                                                                                                 \
+        return fail(nullptr, DCE_ERR_HIP, "no HIP device available: the HIP path is mandatory, there is no CPU fallback");   \
+    if ((id) < 0 || (id) >= device_count()) return fail(nullptr, DCE_ERR_ARG, "device %d out of range (%d devices)", (id), device_count()); \
     DeviceGuard dev_guard_(id);                                                                                              \
     if (dev_guard_.err != hipSuccess) return fail(nullptr, DCE_ERR_HIP, "hipSetDevice(%d) failed: %s", (id), hipGetErrorString(dev_guard_.err))
 

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(GW * 64) void group_place_kernel(const ID* __restri
                                                               int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ place)
 {
     __shared__ int run[GW][GROUPS_MAX];       // a wave's next place in every group
-    __shared__ int base[GROUPS_MAX];          // the chunk's first place in every group
+    __shared__ int base[GROUPS_MAX], before[GROUPS_MAX];   // rows of every group, then its first place; its rows in front of this chunk
     __shared__ int total;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = gridDim.x, me = blockIdx.x;
     const long long lo = (long long)me * chunk;
@@ -67,18 +67,20 @@ __global__ __launch_bounds__(GW * 64) void group_place_kernel(const ID* __restri
     const int wlo = wl < hi ? (int)wl : hi, whi = wl + part < hi ? (int)(wl + part) : hi;
 
     for (int g = lane; g < groups; g += 64) run[wave][g] = 0;
+    for (int g = threadIdx.x; g < groups; g += GW * 64) base[g] = before[g] = 0;
     __syncthreads();
     for (int i = wlo + lane; i < whi; i += 64) { const int k = key_of(ids, i, groups); if (k >= 0) atomicAdd(&run[wave][k], 1); }
+    // rows of every group in all chunks, and in the chunks before this one (sums of whole numbers: any order)
+    if (chunks > 1)
+        for (int i = threadIdx.x; i < chunks * groups; i += GW * 64) {
+            const int c = i / groups, g = i - c * groups, v = work[i];
+            if (v) { atomicAdd(&base[g], v); if (c < me) atomicAdd(&before[g], v); }
+        }
     __syncthreads();
-    // rows of every group in all chunks, and in the chunks before this one
     for (int g = threadIdx.x; g < groups; g += GW * 64) {
-        int before = 0, all = 0;
-        if (chunks > 1) {
-            for (int c = 0; c < chunks; ++c) { const int v = work[(long long)c * groups + g]; all += v; if (c < me) before += v; }
-        } else
-            for (int w = 0; w < GW; ++w) all += run[w][g];
-        base[g] = all;
-        for (int w = 0; w < GW; ++w) { const int v = run[w][g]; run[w][g] = before; before += v; }
+        int at = before[g];
+        for (int w = 0; w < GW; ++w) { const int v = run[w][g]; run[w][g] = at; at += v; }
+        if (chunks == 1) base[g] = at;
     }
     __syncthreads();
     if (wave == 0) {                          // the groups' first places: a scan over 64 groups a step

@@ -39,42 +39,43 @@ def _lib_entries():
     return _entries
 
 
-def _device(*tensors):
-    """The one device of the tensors that are there, and torch's current stream on it."""
-    at = tensors[0].device
-    if at.type != "cuda":
-        raise RuntimeError("deep_contact_estimator_amd runs on MI355X only; there is no CPU path (got a tensor on %s)" % at)
-    grad = torch.is_grad_enabled()
+_grad_on, _raw_stream = torch.is_grad_enabled, torch._C._cuda_getCurrentRawStream
+
+
+def _at(t, what):
+    """The device of a call's first tensor."""
+    dev = t.get_device()
+    if dev < 0:
+        raise RuntimeError(f"{what}: deep_contact_estimator_amd runs on MI355X only; there is no CPU path (got a tensor on {t.device})")
+    return dev
+
+
+def _same(dev, what, *tensors):
+    """... is that of the others too, and none wants a gradient."""
+    grad = _grad_on()
     for t in tensors:
         if t is not None:
-            if t.device != at:
-                raise RuntimeError(f"tensors on {t.device} and on {at}")
+            if t.get_device() != dev:
+                raise RuntimeError(f"{what}: tensors on cuda:{dev} and on {t.device}")
             if grad and t.requires_grad:
-                raise RuntimeError("deep_contact_estimator_amd implements the inference path only: detach the tensor, or call under torch.no_grad()")
-    return at, at.index, torch._C._cuda_getCurrentRawStream(at.index)
+                raise RuntimeError(f"{what}: deep_contact_estimator_amd implements the inference path only: detach the tensor, or call under torch.no_grad()")
 
 
-def _rows(t, what, dims=2):
-    """`t` with its last axis without gaps: itself where it is so already."""
-    if t.dim() != dims:
-        raise RuntimeError(f"{what}: expected {dims} dimensions, got {tuple(t.shape)}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+def _rowed(t):
+    """`t` with its last axis without gaps and rows that do not overlap -- itself where it is so already -- and its strides (of an axis of one
+    entry, whose stride says nothing, what a matrix without gaps has)."""
+    st, shape = t.stride(), t.shape
+    n = shape[-1]
+    if (st[-1] == 1 or n <= 1) and (st[-2] >= n or shape[-2] <= 1):
+        if shape[-2] > 1:
+            return t, st
+        return t, (*st[:-2], max(n, 1), 1)
+    t = t.contiguous()
+    return t, t.stride()
 
 
-def _stride(t, d):
-    """The stride of axis d, of an axis of one entry (whose stride says nothing) what a matrix without gaps has."""
-    if t.shape[d] > 1:
-        return t.stride(d)
-    n = 1
-    for s in t.shape[d + 1:]:
-        n *= s
-    return n
-
-
-def _rowed(t, what, dims=2):
-    """... and rows that do not overlap (an expanded tensor is copied)."""
-    t = _rows(t, what, dims)
-    return t if _stride(t, dims - 2) >= t.shape[-1] else t.contiguous()
+def _vector(t):
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check(rc):
@@ -94,83 +95,101 @@ def quantize(x, rows: int = 1, scale_dtype=E8M0):
         raise RuntimeError(f"quantize: scale_dtype must be float8_e8m0fnu or float32, not {scale_dtype}")
     if rows not in (1, BLOCK):
         raise RuntimeError(f"quantize: a block has 1 row or {BLOCK}, not {rows}")
-    if x.dim() != 2 and (rows == 1 or x.dim() != 3):
-        raise RuntimeError(f"quantize: expected (m, k){' or (groups, n, k)' if rows != 1 else ''}, got {tuple(x.shape)}")
-    at, dev, stream = _device(x)
     dims = x.dim()
-    x = _rowed(x, "quantize", dims)
-    m, k = x.shape[-2], x.shape[-1]
-    batch = x.shape[0] if dims == 3 else 1
-    kb = (k + BLOCK - 1) // BLOCK
-    q = torch.empty(x.shape, dtype=E4M3, device=at)
+    if dims != 2 and (rows == 1 or dims != 3):
+        raise RuntimeError(f"quantize: expected (m, k){' or (groups, n, k)' if rows != 1 else ''}, got {tuple(x.shape)}")
+    dev = _at(x, "quantize")
+    _same(dev, "quantize", x)
+    x, st = _rowed(x)
+    shape = x.shape
+    m, k = shape[-2:]
+    kb = (k + 127) // 128
+    at = x.device
+    q = torch.empty(shape, dtype=E4M3, device=at)
     if rows == 1:
         scale = torch.empty((kb, m), dtype=scale_dtype, device=at)
     else:
-        scale = torch.empty((*x.shape[:-2], (m + BLOCK - 1) // BLOCK, kb), dtype=scale_dtype, device=at)
-    _check(_lib_entries()[0](dev, stream, _QUANTIZE.pack(
-        x.data_ptr(), _stride(x, dims - 2), x.stride(0) if dims == 3 else 0, q.data_ptr(), k, m * k, scale.data_ptr(), m, batch, m, k,
-        _TYPES[x.dtype], _SCALES[scale_dtype], rows, 0)))
+        scale = torch.empty((*shape[:-2], (m + 127) // 128, kb), dtype=scale_dtype, device=at)
+    rc = _lib_entries()[0](dev, _raw_stream(dev), _QUANTIZE.pack(
+        x.data_ptr(), st[-2], st[0] if dims == 3 else 0, q.data_ptr(), k, m * k, scale.data_ptr(), m, shape[0] if dims == 3 else 1, m, k,
+        _TYPES[x.dtype], _SCALES[scale_dtype], rows, 0))
+    if rc:
+        _check(rc)
     return q, scale
 
 
-def _matmul(what, a, a_scale, b, b_scale, bias, relu, out_dtype, out, out_scale, offsets, index, groups):
-    f8 = a.dtype == E4M3
-    if a.dtype != b.dtype or not (f8 or a.dtype == torch.bfloat16):
-        raise RuntimeError(f"{what}: operands must both be bfloat16 or float8_e4m3fn, not {a.dtype} and {b.dtype}")
-    if out_dtype not in _TYPES or (out_dtype == E4M3 and not f8):
-        raise RuntimeError(f"{what}: results of {out_dtype} from {a.dtype}")
-    at, dev, stream = _device(a, b, a_scale, b_scale, bias, out, out_scale, offsets, index)
-    grouped = 3 if groups else 2
-    if a.dim() != 2 or b.dim() != grouped:
-        raise RuntimeError(f"{what}: expected a (rows, k) and b ({'groups, ' if groups else ''}n, k), got {tuple(a.shape)} and {tuple(b.shape)}")
-    a, b = _rowed(a, what), _rowed(b, what, grouped)
-    (rows, k), n = a.shape, b.shape[-2]
+def _matmul(what, a, a_scale, b, b_scale, bias, relu, out_dtype, out, out_scale, offsets, index):
+    kind = a.dtype
+    f8 = kind == E4M3
+    if b.dtype != kind or not (f8 or kind == torch.bfloat16):
+        raise RuntimeError(f"{what}: operands must both be bfloat16 or float8_e4m3fn, not {kind} and {b.dtype}")
+    out_type = _TYPES.get(out_dtype)
+    if out_type is None or (out_type == 2 and not f8):
+        raise RuntimeError(f"{what}: results of {out_dtype} from {kind}")
+    dev = _at(a, what)
+    _same(dev, what, a, b, a_scale, b_scale, bias, out, out_scale, offsets, index)
+    grouped = offsets is not None
+    if a.dim() != 2 or b.dim() != 2 + grouped:
+        raise RuntimeError(f"{what}: expected a (rows, k) and b ({'groups, ' if grouped else ''}n, k), got {tuple(a.shape)} and {tuple(b.shape)}")
+    a, sa = _rowed(a)
+    b, sb = _rowed(b)
+    rows, k = a.shape
+    count, n, kw = b.shape if grouped else (1, *b.shape)
     m = rows if index is None else index.shape[0]
-    if b.shape[-1] != k:
-        raise RuntimeError(f"{what}: a has {k} columns, b {b.shape[-1]}")
-    kb, nb = (k + BLOCK - 1) // BLOCK, (n + BLOCK - 1) // BLOCK
-    count = b.shape[0] if groups else 1
-    scale = E8M0
-    pa = pb = lsa = lsb = gsb = 0
+    if kw != k:
+        raise RuntimeError(f"{what}: a has {k} columns, b {kw}")
+    scale_type = pa = pb = lsa = lsb = gsb = pbias = gbias = py = ls = 0
     if f8:
         if a_scale is None or b_scale is None:
             raise RuntimeError(f"{what}: float8_e4m3fn operands need a_scale and b_scale")
         scale = a_scale.dtype
-        if scale not in _SCALES or b_scale.dtype != scale:
+        scale_type = _SCALES.get(scale)
+        if scale_type is None or b_scale.dtype != scale:
             raise RuntimeError(f"{what}: scales must both be float8_e8m0fnu or float32, not {scale} and {b_scale.dtype}")
-        want = (count, nb, kb) if groups else (nb, kb)
-        if tuple(a_scale.shape) != (kb, rows) or tuple(b_scale.shape) != want:
+        kb, nb = (k + 127) // 128, (n + 127) // 128
+        want = (count, nb, kb) if grouped else (nb, kb)
+        if a_scale.shape != (kb, rows) or b_scale.shape != want:
             raise RuntimeError(f"{what}: expected a_scale {(kb, rows)} and b_scale {want}, got {tuple(a_scale.shape)} and {tuple(b_scale.shape)}")
-        a_scale, b_scale = _rowed(a_scale, what), _rowed(b_scale, what, grouped)
-        pa, pb, lsa, lsb = a_scale.data_ptr(), b_scale.data_ptr(), _stride(a_scale, 0), _stride(b_scale, grouped - 2)
-        gsb = _stride(b_scale, 0) if groups else 0
+        a_scale, st = _rowed(a_scale)
+        lsa = st[0]
+        b_scale, st = _rowed(b_scale)
+        lsb = st[-2]
+        gsb = st[0] if grouped else 0
+        pa, pb = a_scale.data_ptr(), b_scale.data_ptr()
     elif a_scale is not None or b_scale is not None:
         raise RuntimeError(f"{what}: bfloat16 operands have no scales")
-    pbias = gbias = 0
     if bias is not None:
-        want = (count, n) if groups else (n,)
-        if bias.dtype != torch.float32 or tuple(bias.shape) != want:
+        want = (count, n) if grouped else (n,)
+        if bias.dtype != torch.float32 or bias.shape != want:
             raise RuntimeError(f"{what}: bias must be float32 {want}, got {bias.dtype} {tuple(bias.shape)}")
-        bias = _rows(bias, what, len(want))
-        pbias, gbias = bias.data_ptr(), _stride(bias, 0) if groups else 0
+        st = bias.stride()
+        if st[-1] != 1 and n > 1:
+            bias = bias.contiguous()
+            st = bias.stride()
+        pbias, gbias = bias.data_ptr(), st[0] if grouped else 0
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=at)
-    elif out.dtype != out_dtype or tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1) or _stride(out, 0) < n:
-        raise RuntimeError(f"{what}: out must be a {out_dtype} ({m},{n}) tensor whose rows have no gaps and do not overlap")
-    py = ls = 0
-    if out_dtype == E4M3:
+        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        ldy = n
+    else:
+        ldy, step = out.stride() if out.dim() == 2 else (0, 0)
+        if out.shape == (m, n) and m <= 1:
+            ldy = n
+        if out.dtype != out_dtype or out.shape != (m, n) or (n > 1 and step != 1) or ldy < n:
+            raise RuntimeError(f"{what}: out must be a {out_dtype} ({m},{n}) tensor whose rows have no gaps and do not overlap")
+    if out_type == 2:
         if out_scale is None:
-            out_scale = torch.empty((nb, m), dtype=scale, device=at)
-        elif out_scale.dtype != scale or tuple(out_scale.shape) != (nb, m) or not out_scale.is_contiguous():
+            out_scale = torch.empty((nb, m), dtype=scale, device=a.device)
+        elif out_scale.dtype != scale or out_scale.shape != (nb, m) or not out_scale.is_contiguous():
             raise RuntimeError(f"{what}: out_scale must be a contiguous {scale} ({nb},{m}) tensor")
         py, ls = out_scale.data_ptr(), m
     elif out_scale is not None:
         raise RuntimeError(f"{what}: out_scale belongs to float8_e4m3fn results")
-    _check(_lib_entries()[1](dev, stream, _MATMUL.pack(
-        a.data_ptr(), _stride(a, 0), pa, lsa, b.data_ptr(), _stride(b, grouped - 2), _stride(b, 0) if groups else 0, pb, lsb, gsb, pbias, gbias,
-        out.data_ptr(), _stride(out, 0), py, ls, offsets.data_ptr() if groups else 0, 0 if index is None else index.data_ptr(), rows, m, n, k,
-        count, _TYPES[a.dtype], _SCALES[scale], _TYPES[out_dtype], 1 if relu else 0, 0)))
-    return (out, out_scale) if out_dtype == E4M3 else out
+    rc = _lib_entries()[1](dev, _raw_stream(dev), _MATMUL.pack(
+        a.data_ptr(), sa[0], pa, lsa, b.data_ptr(), sb[-2], sb[0] if grouped else 0, pb, lsb, gsb, pbias, gbias, out.data_ptr(), ldy, py, ls,
+        offsets.data_ptr() if grouped else 0, 0 if index is None else index.data_ptr(), rows, m, n, k, count, _TYPES[kind], scale_type, out_type, 1 if relu else 0, 0))
+    if rc:
+        _check(rc)
+    return (out, out_scale) if out_type == 2 else out
 
 
 def matmul_fp8(a, a_scale, b, b_scale, bias=None, relu: bool = False, out_dtype=torch.bfloat16, out=None, out_scale=None):
@@ -179,7 +198,7 @@ def matmul_fp8(a, a_scale, b, b_scale, bias=None, relu: bool = False, out_dtype=
     rounded once to out_dtype: float32, bfloat16, or float8_e4m3fn -- then (q, scale) with a power of two for every 128 columns of a
     row, in the operands' scale dtype: the next product's a and a_scale.  Any sizes and row strides; rows that start at multiples of
     16 bytes run fastest."""
-    return _matmul("matmul_fp8", a, a_scale, b, b_scale, bias, relu, out_dtype, out, out_scale, None, None, 0)
+    return _matmul("matmul_fp8", a, a_scale, b, b_scale, bias, relu, out_dtype, out, out_scale, None, None)
 
 
 def matmul_grouped(a, b, offsets, index=None, a_scale=None, b_scale=None, bias=None, relu: bool = False, out_dtype=torch.bfloat16, out=None,
@@ -191,14 +210,14 @@ def matmul_grouped(a, b, offsets, index=None, a_scale=None, b_scale=None, bias=N
     a row of zeros; rows that no group covers stay as they were in `out` (in a fresh result they hold nothing of use)."""
     if b.dim() != 3 or not 1 <= b.shape[0] <= GROUPS_MAX:
         raise RuntimeError(f"matmul_grouped: expected b (1 .. {GROUPS_MAX} groups, n, k), got {tuple(b.shape)}")
-    if offsets.dtype != torch.int32 or tuple(offsets.shape) != (b.shape[0] + 1,):
+    if offsets.dtype != torch.int32 or offsets.shape != (b.shape[0] + 1,):
         raise RuntimeError(f"matmul_grouped: offsets must be int32 ({b.shape[0] + 1},), got {offsets.dtype} {tuple(offsets.shape)}")
-    offsets = _rows(offsets, "matmul_grouped", 1)
+    offsets = _vector(offsets)
     if index is not None:
         if index.dtype != torch.int32 or index.dim() != 1:
             raise RuntimeError(f"matmul_grouped: index must be int32 (m,), got {index.dtype} {tuple(index.shape)}")
-        index = _rows(index, "matmul_grouped", 1)
-    return _matmul("matmul_grouped", a, a_scale, b, b_scale, bias, relu, out_dtype, out, out_scale, offsets, index, True)
+        index = _vector(index)
+    return _matmul("matmul_grouped", a, a_scale, b, b_scale, bias, relu, out_dtype, out, out_scale, offsets, index)
 
 
 def group_rows(ids, groups: int):
@@ -209,18 +228,20 @@ def group_rows(ids, groups: int):
     groups = int(groups)
     if not 1 <= groups <= GROUPS_MAX:
         raise RuntimeError(f"group_rows: 1 .. {GROUPS_MAX} groups, not {groups}")
-    at, dev, stream = _device(ids)
-    ids = _rows(ids, "group_rows", 1)
+    dev = _at(ids, "group_rows")
+    ids = _vector(ids)
     n = ids.shape[0]
     lib = _lib_entries()
     need = lib[3](n, groups)
     if need < 0:
         _check(need)
-    offsets = torch.empty(groups + 1, dtype=torch.int32, device=at)
-    order, place = torch.empty((2, n), dtype=torch.int32, device=at).unbind(0)
-    work = torch.empty(need, dtype=torch.int32, device=at) if need else None
-    _check(lib[2](dev, stream, ids.data_ptr(), ids.element_size(), n, groups, offsets.data_ptr(), order.data_ptr(), place.data_ptr(),
-                  work.data_ptr() if need else None))
+    made = torch.empty(groups + 1 + 2 * n + need, dtype=torch.int32, device=ids.device)
+    offsets, order, place, work = made.split_with_sizes((groups + 1, n, n, need))
+    p = made.data_ptr()
+    rc = lib[2](dev, _raw_stream(dev), ids.data_ptr(), ids.element_size(), n, groups, p, p + 4 * (groups + 1), p + 4 * (groups + 1 + n),
+                p + 4 * (groups + 1 + 2 * n) if need else None)
+    if rc:
+        _check(rc)
     return offsets, order, place
 
 
@@ -229,15 +250,16 @@ def decide(logits, index=None):
     contact_cnn.predict returns them; an index outside the rows gives NaN logits and class 0."""
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.shape[1] != 16:
         raise RuntimeError(f"decide: expected float32 (rows, 16) logits, got {logits.dtype} {tuple(logits.shape)}")
-    at, dev, stream = _device(logits, index)
-    logits = logits.contiguous()
+    dev = _at(logits, "decide")
+    _same(dev, "decide", logits, index)
+    logits, at = logits.contiguous(), logits.device
     if index is not None:
         if index.dtype != torch.int32 or index.dim() != 1:
             raise RuntimeError(f"decide: index must be int32 (n,), got {index.dtype} {tuple(index.shape)}")
-        index = _rows(index, "decide", 1)
+        index = _vector(index)
     n = logits.shape[0] if index is None else index.shape[0]
     out = {"logits": torch.empty((n, 16), dtype=torch.float32, device=at), "pred": torch.empty((n,), dtype=torch.int32, device=at),
            "contacts": torch.empty((n, 4), dtype=torch.uint8, device=at)}
-    _check(_lib_entries()[4](dev, stream, logits.data_ptr(), logits.shape[0], None if index is None else index.data_ptr(), n,
+    _check(_lib_entries()[4](dev, _raw_stream(dev), logits.data_ptr(), logits.shape[0], None if index is None else index.data_ptr(), n,
                              out["logits"].data_ptr(), out["pred"].data_ptr(), out["contacts"].data_ptr()))
     return out
