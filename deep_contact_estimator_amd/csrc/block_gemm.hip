@@ -13,12 +13,6 @@
 #include "block_ops.h"
 #include <cmath>
 
-#ifndef FORCE
-#define FORCE -1
-#endif
-#ifndef ROWS_T
-#define ROWS_T 64
-#endif
 namespace dce {
 
 namespace {
@@ -123,8 +117,12 @@ template <int IN, bool EXACT> struct Scale {
 // are good to 1e-8.
 //
 // One row of blocks at a time: instructions that add to the same sums are as far apart as the row is long (a dependent one waits for its predecessor).
+// Where the matrix instruction can apply the scales (or there are none) it adds to `acc`; otherwise the block's sums go to `part` and fold_row brings
+// them home -- behind the next row's matrix instructions, which hide it.
+template <int IN, bool EXACT> constexpr bool FOLDS = IN != IN_BF16 && (EXACT || IN == IN_F8_F32);
+
 template <int IN, bool EXACT, int NT>
-__device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> (&w)[NT], const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
+__device__ __forceinline__ void mfma_row(f32x4 (&acc)[NT], f32x4 (&part)[NT], const Frag<IN, EXACT> (&w)[NT], const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
 {
     if constexpr (IN == IN_BF16) {
 #pragma unroll
@@ -133,30 +131,35 @@ __device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> 
         for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j].c1), __builtin_bit_cast(bf16x8, x.c1), acc[j], 0, 0, 0);
     } else if constexpr (EXACT) {
         const float z = IN == IN_F8_E8 ? sc.start : 0.f;
-        f32x4 part[NT];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int j = 0; j < NT; ++j) part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j].h[k], x.h[k], k ? part[j] : f32x4{z, z, z, z}, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = IN == IN_F8_E8 ? acc[j][i] + ldexpf(part[j][i], sc.e) : fmaf(part[j][i], sc.s, acc[j][i]);
     } else {
         const i32x8 xv = __builtin_shufflevector(x.c0, x.c1, 0, 1, 2, 3, 4, 5, 6, 7);
-        f32x4 part[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const i32x8 wv = __builtin_shufflevector(w[j].c0, w[j].c1, 0, 1, 2, 3, 4, 5, 6, 7);
             if constexpr (IN == IN_F8_E8) acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[j], 0, 0, 0, sc.ew, 0, sc.ex);
             else part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 127, 0, 127);
         }
-        if constexpr (IN == IN_F8_F32)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[j][i], sc.s, acc[j][i]);
     }
+}
+template <int IN, bool EXACT, int NT>
+__device__ __forceinline__ void fold_row(f32x4 (&acc)[NT], const f32x4 (&part)[NT], const Scale<IN, EXACT>& sc)
+{
+    if constexpr (FOLDS<IN, EXACT>)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = IN == IN_F8_E8 ? acc[j][i] + ldexpf(part[j][i], sc.e) : fmaf(part[j][i], sc.s, acc[j][i]);
+}
+template <int IN, bool EXACT, int NT>
+__device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> (&w)[NT], const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
+{
+    f32x4 part[NT];
+    mfma_row<IN, EXACT, NT>(acc, part, w, x, sc);
+    fold_row<IN, EXACT, NT>(acc, part, sc);
 }
 
 __device__ __forceinline__ unsigned short to_bf16(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
@@ -428,23 +431,31 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
             read(next);
         }
         Frag<IN, EXACT> w[NT];
+        constexpr bool LATE = MT * NT < 16;                                   // (a second row of block sums would spill)
+        f32x4 part[2][NT];
+        Scale<IN, EXACT> sc[2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) w[j].set(f.w0[j], f.w1[j]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             Frag<IN, EXACT> x;
             x.set(f.x0[i], f.x1[i]);
-            Scale<IN, EXACT> sc;
-            if (PS) sc.set(f.sw, f.sx[i]);
-            mac_row<IN, EXACT, NT>(acc[i], w, x, sc);
+            if (PS) sc[i & 1].set(f.sw, f.sx[i]);
+            mfma_row<IN, EXACT, NT>(acc[i], part[i & 1], w, x, sc[i & 1]);
             if (s + NBUF < steps) {                                           // requests between the instructions, some behind each row: the pipe is busy while they are issued
 #pragma unroll
-                for (int j = 0; j < NT; ++j) asm volatile("" :: "v"(acc[i][j]));
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (FOLDS<IN, EXACT>) asm volatile("" :: "v"(part[i & 1][j]));
+                    else asm volatile("" :: "v"(acc[i][j]));
+                }
                 __builtin_amdgcn_sched_barrier(0);
                 bring(s + NBUF, i * ALL / MT, (i + 1) * ALL / MT);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (LATE && i > 0) fold_row<IN, EXACT, NT>(acc[i - 1], part[(i - 1) & 1], sc[(i - 1) & 1]);
+            if (!LATE) fold_row<IN, EXACT, NT>(acc[i], part[i & 1], sc[i & 1]);
         }
+        if (LATE) fold_row<IN, EXACT, NT>(acc[MT - 1], part[(MT - 1) & 1], sc[(MT - 1) & 1]);
     };
     // (step 0 alone: NBUF steps are under way, and one fewer behind it than `arrive` counts on)
     if (NBUF - 1 < steps) wait_all_but<(NBUF - 1) * (T::PIECES + PS)>();
@@ -688,11 +699,12 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             phase_end();
             // ---- M
             __builtin_amdgcn_s_setprio(1);
+            f32x4 part[2][NT];
+            Scale<IN, EXACT> sc[2];
 #pragma unroll
             for (int i = 0; i < XG; ++i) {
-                Scale<IN, EXACT> sc;
-                if (PS) sc.set(sw, sv[i]);
-                mac_row<IN, EXACT, NT>(acc[h * XG + i], w, x[i], sc);
+                if (PS) sc[i & 1].set(sw, sv[i]);
+                mfma_row<IN, EXACT, NT>(acc[h * XG + i], part[i & 1], w, x[i], sc[i & 1]);
                 // requests between the instructions, a few behind each row: the pipe is busy while they are issued
                 int next = s + 2;
                 bool ask;
@@ -705,14 +717,17 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
                 }
                 if (ask && i < XG - 1) {
                     const int to = NBUF == 2 ? next & 1 : grp == 0 ? buf2 : buf;
-                    pin(acc[h * XG + i]);
+                    if constexpr (FOLDS<IN, EXACT>) pin(part[i & 1]);
+                    else pin(acc[h * XG + i]);
                     __builtin_amdgcn_sched_barrier(0);
                     if (NBUF == 3) bring(next, to, i * ALL / (XG - 1), (i + 1) * ALL / (XG - 1));
                     else if (h == 0) bring(next, to, i * PB / (XG - 1), (i + 1) * PB / (XG - 1));
                     else bring(next, to, PB + i * (PS + PA) / (XG - 1), PB + (i + 1) * (PS + PA) / (XG - 1));
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                if (i > 0) fold_row<IN, EXACT, NT>(acc[h * XG + i - 1], part[(i - 1) & 1], sc[(i - 1) & 1]);
             }
+            fold_row<IN, EXACT, NT>(acc[h * XG + XG - 1], part[(XG - 1) & 1], sc[(XG - 1) & 1]);
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int i = 0; i < XG; ++i) pin(acc[h * XG + i]);
@@ -865,46 +880,62 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
     return hipGetLastError();
 }
 
+// Which kernel: the one with the least estimated time, 2 us + rounds of 256 tiles x (a tile's beginning and end + its steps).  The microseconds below are
+// fitted to runs on 1 .. 32768 rows of 2048 x 4736 and 512 x 2048 and to grouped ones (a graph of 20 calls each; us):
+//
+//   rows            e4m3 to bf16: few rows   32 x 128   64 x 128   128 x 128   128 x 256   192 x 256   256 x 256
+//        1                             5.7       15.5       19.4        26.3        30.1                    50.7
+//       32                             7.4       15.7       19.4        26.3        30.4                    50.7
+//      128                            19.2       16.6                               30.7
+//     1024                                       33.8       22.4        28.8        33.4                    52.6
+//     2048                                       62.3       41.7        30.5        34.7        48.2        54.1
+//     4096                                      119.5       78.4        56.9        43.3        53.7        56.1
+//     5000                                                                          69.8        52.7        58.4
+//    32768                                       1015        652         452         303         301         254
 template <int IN, int OUT>
 hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
-    const int mean = (p.m + p.groups - 1) / p.groups;                         // rows a group
-    if constexpr (OUT != OUT_E4M3)
-        if (p.a_rows > 0 && p.kbytes > 0 && mean <= ROWS_T) {
-            if (mean <= 16) return launch_rows<IN, OUT, 1, 3>(p, st);
-            return launch_rows<IN, OUT, 2, 2>(p, st);
-        }
+    constexpr bool EXACT = OUT == OUT_F32;
+    constexpr int F = !FOLDS<IN, EXACT> ? 0 : !EXACT ? 1 : 2;                 // scales for the matrix instruction (or none) | block sums folded | e4m3 as fp16
+    if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
-    const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // (32-bit offsets)
-    if (!aligned || !near || p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
-    const bool whole = p.kbytes % KROW == 0;
-    // what a row of tiles' steps cost: rounds of a tile on every CU, times its step
-    const double rows = p.offsets ? p.m + 0.5 : p.m;
-    auto cost = [&](int bm, int bn, double step) {
-        const double tiles = (p.offsets ? (double)p.m / bm + 0.5 * (p.groups < p.m ? p.groups : p.m) : (double)((p.m + bm - 1) / bm)) * ((p.n + bn - 1) / bn);
-        return ceil(tiles / 256.0) * step;
+    const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // the ring's and the phased kernel's 32-bit offsets
+    const bool dma = aligned && near, whole = dma && p.kbytes % KROW == 0;
+    const double steps = (p.kbytes + KROW - 1) / KROW;
+    enum { ROWS16, ROWS32, ANY, R32, R64, R128, P128, P192, P256 };
+    int best = -1;
+    double least = 0;
+    auto offer = [&](int kernel, bool can, int bm, int bn, double edge, double step) {
+        if (!can) return;
+        const double rows = p.offsets ? (double)p.m / bm + 0.5 * (p.groups < p.m ? p.groups : p.m) : (double)((p.m + bm - 1) / bm);   // (a group's last tile is half full)
+        const double us = 2 + ceil(rows * ((p.n + bn - 1) / bn) / 256) * (edge + steps * step);
+        if (best < 0 || us < least) { best = kernel; least = us; }
     };
-    (void)rows;
-    constexpr bool F16 = OUT == OUT_F32 && IN != IN_BF16;                     // e4m3 as fp16
-    const double c32 = cost(32, 128, 0.30), c64 = cost(64, 128, 0.36), c128 = F16 ? 1e30 : cost(128, 128, 0.5);
-    const double w128 = whole ? cost(128, 256, F16 ? 1.3 : 0.9) : 1e30, w256 = whole && !F16 ? cost(256, 256, 1.5) : 1e30;
-    double best = c32; int pick = FORCE;
-    if (pick < 0) {
-        pick = 0;
-        if (c64 <= best) { best = c64; pick = 1; }
-        if (c128 <= best) { best = c128; pick = 2; }
-        if (w128 <= best) { best = w128; pick = 3; }
-        if (w256 <= best) { best = w256; pick = 4; }
+    offer(ROWS16, OUT != OUT_E4M3, 16, 16, 1.5, aligned ? 0.13 : 0.2);
+    offer(ROWS32, OUT != OUT_E4M3, 32, 16, 1.5, aligned ? 0.17 : 0.25);
+    offer(ANY, !dma, 32, 128, 2, 1.3);
+    offer(R32, dma, 32, 128, 2, F == 0 ? 0.40 : F == 1 ? 0.46 : 0.63);
+    offer(R64, dma, 64, 128, 2, F == 0 ? 0.50 : F == 1 ? 0.58 : 0.92);
+    offer(R128, dma && F == 0, 128, 128, 3, 0.72);                            // (folding does not fit its registers)
+    offer(P128, whole, 128, 256, 4, F == 0 ? 1.06 : F == 1 ? 1.28 : 1.85);
+    offer(P192, whole && F < 2, 192, 256, 4, F == 0 ? 1.35 : 1.45);
+    offer(P256, whole && F < 2, 256, 256, 5, F == 0 ? 1.65 : 2.05);
+    if constexpr (OUT != OUT_E4M3) {
+        if (best == ROWS16) return launch_rows<IN, OUT, 1, 3>(p, st);
+        if (best == ROWS32) return launch_rows<IN, OUT, 2, 2>(p, st);
     }
-    if (pick >= 3 && !whole) pick = 2;
-    if (F16 && pick >= 4) pick = 3;
-    if (F16 && pick == 2) pick = 1;
-    if constexpr (!F16) if (pick == 5) return launch_phased<IN, OUT, Phased<2, 4, 6, 4, 2>>(p, st);
-    if constexpr (!F16) if (pick == 4) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
-    if (pick == 3) return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
-    if constexpr (!F16) if (pick == 2) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);
-    if (pick == 1) return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 5>>(p, st);
-    return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 6>>(p, st);
+    if constexpr (F == 0)
+        if (best == R128) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);
+    if constexpr (F < 2) {
+        if (best == P192) return launch_phased<IN, OUT, Phased<2, 4, 6, 4, 2>>(p, st);
+        if (best == P256) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
+    }
+    switch (best) {
+    case R32: return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 6>>(p, st);
+    case R64: return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 5>>(p, st);
+    case P128: return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
+    default: return launch_any<IN, OUT>(p, st);
+    }
 }
 
 template <int IN>
