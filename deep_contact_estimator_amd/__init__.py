@@ -7,4 +7,13 @@ built library; using the model does (there is no CPU fallback).
 from .contact_cnn import contact_cnn, load_checkpoint          # noqa: F401
 from . import synth                                              # noqa: F401
 
-__all__ = ["contact_cnn", "load_checkpoint", "synth"]
+__all__ = ["contact_cnn", "contact_bank", "load_checkpoint", "ops", "synth"]
+
+
+def __getattr__(name):                                             # (these import torch: only when asked for)
+    import importlib
+    if name == "ops":
+        return importlib.import_module(".ops", __name__)
+    if name == "contact_bank":
+        return importlib.import_module(".bank", __name__).contact_bank
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

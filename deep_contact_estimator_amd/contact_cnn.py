@@ -25,7 +25,7 @@ from .synth import STATE_DICT_SHAPES
 
 WINDOW, CHANNELS, CLASSES = 150, 54, 16
 PACKED_ROW = 68                        # include/dce.h DCE_PACKED_ROW: 16 fp32 logits + 4 contact bits
-PRECISIONS = {"fp32": 0, "bf16_fc": 1, "fp32_split": 2, "fp32_f16x2": 3}   # fp32_split: fc.0 on three-term bf16 operands (include/dce.h DCE_FP32_SPLIT)
+PRECISIONS = {"fp32": 0, "bf16_fc": 1, "fp32_split": 2, "fp32_f16x2": 3, "fp8_fc": 4}   # fp32_split: fc.0 on three-term bf16 operands (include/dce.h DCE_FP32_SPLIT)
 
 
 def _is_torch(x) -> bool:
@@ -384,12 +384,34 @@ class contact_cnn:
         n = a.shape[0]
         out = {"h2": np.empty((n, 512), np.float32), "logits": np.empty((n, CLASSES), np.float32)}
         act = np.uint16 if self._precision == "bf16_fc" else np.float32     # bf16-FC mode: the bf16 bit patterns
-        out["feat"] = np.empty((n, 4736), act)
-        out["h1"] = np.empty((n, 2048), act)
+        if self._precision != "fp8_fc":                                     # (there they are e4m3 with scales: not handed out)
+            out["feat"] = np.empty((n, 4736), act)
+            out["h1"] = np.empty((n, 2048), act)
         p = lambda k: out[k].ctypes.data_as(C.c_void_p) if k in out else None
         _lib.check(self._lib.dce_set_stream(self._ctx, None, 1), self._ctx)
         _lib.check(self._lib.dce_forward_taps(self._ctx, a.ctypes.data_as(C.c_void_p), n, 0,
                                               p("feat"), p("h1"), p("h2"), p("logits")), self._ctx)
+        return out
+
+    def features(self, x, raw_sequence: bool = False):
+        """The conv stack alone (dce_features): CUDA (n,150,54) z-scored windows, or a raw (T,54) sequence, -> (n,4736) bfloat16, value (t, c) of
+        a window at t * 128 + c -- for FC layers of one's own (ops.py, contact_bank).  Precisions bf16_fc and fp8_fc."""
+        import torch
+        if not (_is_torch(x) and x.is_cuda):
+            raise RuntimeError("features: expected a CUDA tensor")
+        if raw_sequence:
+            if x.ndim != 2 or x.shape[1] != CHANNELS:
+                raise RuntimeError(f"expected a (T,{CHANNELS}) sequence, got {tuple(x.shape)}")
+        else:
+            self._check_windows(x)
+        self._finalize()
+        if x.device.index != self._dev_index:
+            raise RuntimeError(f"input on cuda:{x.device.index}, model on cuda:{self._dev_index}")
+        x = x.contiguous().float()
+        n = max(x.shape[0] - (WINDOW - 1) if raw_sequence else x.shape[0], 0)
+        out = torch.empty((n, 4736), dtype=torch.bfloat16, device=x.device)
+        self._torch_stream(x)
+        _lib.check(self._lib.dce_features(self._ctx, C.c_void_p(x.data_ptr()) if n else None, n, int(bool(raw_sequence)), C.c_void_p(out.data_ptr()) if n else None), self._ctx)
         return out
 
     CONV_KERNELS = {"wino2": 0, "wino1x8": 1, "half": 2, "quarter": 3, "direct": 4, "wino1x4": 5, "wino2rt4": 6, "x3": 7, "h2": 8}

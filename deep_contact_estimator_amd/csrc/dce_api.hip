@@ -4,6 +4,7 @@
 //   conv_stack (z-score+conv1..4)  ->  fc_gemm (fc.0)  ->  fc_gemm (fc.3)  ->  fc3_tail (fc.6+argmax+bits)
 // No exception or abort crosses the boundary; every failure is a negative dce_status plus a message.
 #include "dce_ctx.h"
+#include "block_ops.h"
 #include <chrono>
 #include <cfloat>
 #include <climits>
@@ -337,8 +338,8 @@ struct GateScope {
 // table for DESIGN.md's appendix.
 enum class Conv { WinoF32, WinoBf16, X2Bf16, H2, H2F32, H2Bf16,
                   WinoPlanes, X3Planes, X3F32, PairPlanes, PairBf16 };                     // (second line: experiments build)
-enum class Fc0 { F32, Gemv, Bf16, H2, X3 };
-enum class Fc3 { F32, Gemv, Fused, Bf16, FusedBf16, FusedH2, H2, FusedX3, FusedBf16K };
+enum class Fc0 { F32, Gemv, Bf16, H2, F8, X3 };
+enum class Fc3 { F32, Gemv, Fused, Bf16, FusedBf16, FusedH2, H2, F8, FusedX3, FusedBf16K };
 struct Plan {
     Conv conv; int permk;                 // permk: features (and fc.0's weights) in the K order t' * 128 + c; 2: from persistent workgroups (experiments)
     Fc0 fc0; bool split3;                 // split3 (experiments): fp32 features split by a kernel of their own in front of fc_gemm_x3
@@ -375,8 +376,21 @@ int64_t plan_threshold(const Tuning& tu, Thr t)
 Plan choose_plan_experiments(const dce_ctx* c, int zscore, int64_t n);
 #endif
 
+// DCE_FP8_FC (both builds): DCE_BF16_FC's conv stack, the features quantized behind it, e4m3 products (their kernels resolve by size: block_gemm.hip)
+Plan choose_plan_f8(const dce_ctx* c, int zscore, int64_t n)
+{
+    const Tuning& tu = tune();
+    const bool online = c->src_row_dev != nullptr;
+    Plan p{Conv::X2Bf16, 0, Fc0::F8, false, Fc3::F8, n, false, false, false};
+    if (n >= plan_threshold(tu, T_BF16H2) && !online && tu.bf16_conv_h2 && tu.x3_conv && c->pkh2.w[0] && c->fc1w_f8p) p.conv = Conv::H2Bf16;
+    else if (!tu.x3_conv || n < tu.x3_bf16_min || (online && !zscore)) p.conv = Conv::WinoBf16;
+    p.permk = p.conv == Conv::H2Bf16 || (p.conv == Conv::X2Bf16 && tu.x3_permk && c->fc1w_f8p) ? 1 : 0;
+    return p;
+}
+
 Plan choose_plan(const dce_ctx* c, int zscore, int64_t n)
 {
+    if (c->precision == DCE_FP8_FC) return choose_plan_f8(c, zscore, n);
     const Tuning& tu = tune();                                        // (bound by run_chunk: the context's switches)
     Plan p{Conv::WinoF32, 0, Fc0::F32, false, Fc3::F32, 0, false, false, false};
     const bool online = c->src_row_dev != nullptr;                    // the online graph: the window start lives in device memory
@@ -502,6 +516,77 @@ int ensure_fc1w_x3(dce_ctx* c)
 }
 #endif
 
+// DCE_FP8_FC's operands live in the halves of `feat` and `h1` that 16-bit values leave free: features e4m3 behind the bf16 ones, their scales behind those
+// (37 bytes a row); h1 e4m3 and its scales (16 bytes a row) in h1.
+unsigned char* f8_features(const dce_ctx* c) { return reinterpret_cast<unsigned char*>(c->feat) + (size_t)c->max_batch * FEAT * 2; }
+unsigned char* f8_feature_scales(const dce_ctx* c) { return f8_features(c) + (size_t)c->max_batch * FEAT; }
+unsigned char* f8_h1_scales(const dce_ctx* c) { return reinterpret_cast<unsigned char*>(c->h1) + (size_t)c->max_batch * FC1; }
+static_assert(FEAT % 128 == 0 && FC1 % 128 == 0 && FEAT * 4 >= FEAT * 3 + FEAT / 128 && FC1 * 4 >= FC1 + FC1 / 128, "they fit");
+
+QuantArgs features_f8(const dce_ctx* c, int64_t n)
+{
+    QuantArgs a{};
+    a.x = reinterpret_cast<const char*>(c->feat); a.x_row = FEAT * 2;
+    a.q = f8_features(c); a.q_row = FEAT;
+    a.s = f8_feature_scales(c); a.s_block = n;
+    a.rows = n; a.k = FEAT; a.kblocks = FEAT / BLK; a.units = n * a.kblocks;
+    return a;
+}
+ProductArgs fc0_f8(const dce_ctx* c, int64_t n, int permk)
+{
+    ProductArgs p{};
+    p.a = reinterpret_cast<const char*>(f8_features(c)); p.a_row = FEAT; p.a_rows = n; p.sa = f8_feature_scales(c); p.sa_block = n;
+    p.b = reinterpret_cast<const char*>(permk ? c->fc1w_f8p : c->fc1w_f8); p.b_row = FEAT; p.sb = permk ? c->fc1s_f8p : c->fc1s_f8; p.sb_row = FEAT / BLK;
+    p.bias = c->fc1b; p.relu = 1;
+    p.y = reinterpret_cast<char*>(c->h1); p.y_row = FC1; p.ys = f8_h1_scales(c); p.ys_block = n;
+    p.m = (int)n; p.n = FC1; p.kbytes = FEAT; p.groups = 1;
+    return p;
+}
+ProductArgs fc3_f8(const dce_ctx* c, int64_t n)
+{
+    ProductArgs p{};
+    p.a = reinterpret_cast<const char*>(c->h1); p.a_row = FC1; p.a_rows = n; p.sa = f8_h1_scales(c); p.sa_block = n;
+    p.b = reinterpret_cast<const char*>(c->fc2w_f8); p.b_row = FC1; p.sb = c->fc2s_f8; p.sb_row = FC1 / BLK;
+    p.bias = c->fc2b; p.relu = 1;
+    p.y = reinterpret_cast<char*>(c->h2); p.y_row = FC2 * 4;
+    p.m = (int)n; p.n = FC2; p.kbytes = FC1; p.groups = 1;
+    return p;
+}
+
+// ... and its weights, quantized on the device from the fp32 ones (w1p: fc.0 in the feature order t' * 128 + c, on the host; empty: not wanted)
+int quantize_weights_f8(dce_ctx* c, const std::vector<float>& w1p)
+{
+    const size_t n1 = (size_t)FC1 * FEAT, s1 = (size_t)(FC1 / BLK) * (FEAT / BLK), n2 = (size_t)FC2 * FC1, s2 = (size_t)(FC2 / BLK) * (FC1 / BLK);
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t total = 2 * (n1 + up(s1)) + n2 + up(s2);
+    if (c->f8) { HIP_TRY(c, dev_free(c->f8)); c->f8 = nullptr; }
+    HIP_TRY(c, dev_alloc(&c->f8, guard_of(c, 8), total));
+    unsigned char *w1 = c->f8, *w1q = w1 + n1 + up(s1), *w2 = w1q + n1 + up(s1);
+    auto run = [&](const float* x, unsigned char* q, int rows, int k) {
+        QuantArgs a{};
+        a.x = reinterpret_cast<const char*>(x); a.x_row = (long long)k * 4;
+        a.q = q; a.q_row = k;
+        a.s = q + (size_t)rows * k; a.s_block = k / BLK;
+        a.rows = rows; a.k = k; a.kblocks = k / BLK; a.units = (long long)rows * a.kblocks;
+        return launch_quantize(a, 0, 1, BLK, 1, c->stream);
+    };
+    HIP_TRY(c, run(c->fc1w, w1, FC1, FEAT));
+    HIP_TRY(c, run(c->fc2w, w2, FC2, FC1));
+    c->fc1w_f8 = w1; c->fc1s_f8 = w1 + n1; c->fc2w_f8 = w2; c->fc2s_f8 = w2 + n2;
+    if (!w1p.empty()) {
+        float* tmp = nullptr;
+        HIP_TRY(c, hipMalloc(reinterpret_cast<void**>(&tmp), n1 * sizeof(float)));
+        hipError_t e = hipMemcpy(tmp, w1p.data(), n1 * sizeof(float), hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = run(tmp, w1q, FC1, FEAT);
+        if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+        (void)hipFree(tmp);
+        if (e != hipSuccess) return fail(c, DCE_ERR_HIP, "quantizing fc.0's weights failed: %s", hipGetErrorString(e));
+        c->fc1w_f8p = w1q; c->fc1s_f8p = w1q + n1;
+    }
+    HIP_TRY(c, hipStreamSynchronize(c->stream));
+    return DCE_OK;
+}
+
 // One chunk (n <= max_batch) of the path, everything on device.
 //   src: raw sequence rows (zscore=1) or pre-normalised windows (zscore=0)
 int run_plan(dce_ctx* c, const Plan& p, const float* src, int zscore, int64_t n,
@@ -563,6 +648,11 @@ int run_plan(dce_ctx* c, const Plan& p, const float* src, int zscore, int64_t n,
 #else
       case Fc0::X3: return fail(c, DCE_ERR_STATE, "internal: fc.0 on three-term operands is an experiments-build kernel");
 #endif
+      case Fc0::F8:
+          HIP_TRY(c, launch_quantize(features_f8(c, n), 1, 1, 1, 1, st));
+          HIP_TRY(c, launch_product(fc0_f8(c, n, p.permk), IN_F8_E8, OUT_E4M3, st));
+          plan_note("quantize_e4m3"); plan_note("fc0_e4m3");
+          break;
       case Fc0::Bf16: HIP_TRY(c, launch_fc_gemm_bf16(c->feat, p.permk ? c->fc1w_bf16p : c->fc1w_bf16, c->fc1b, c->h1, 1, n, FC1, FEAT, 1, st)); break;
       case Fc0::H2:
           if (p.fc3 == Fc3::FusedH2 || p.fc3 == Fc3::H2) HIP_TRY(c, launch_fc_gemm_h2(c->feat3, c->feat_scale, c->fc1w_h2, c->fc1_sw, c->fc1b, c->h1, n, FC1, FEAT, 1, st, c->h1h, c->h1_scale, c->fc1_eW, c->fc1_eB));
@@ -572,6 +662,7 @@ int run_plan(dce_ctx* c, const Plan& p, const float* src, int zscore, int64_t n,
     const int64_t nf = p.fused_rows;
     { Timer t(c, 2);
       switch (p.fc3) {
+      case Fc3::F8: HIP_TRY(c, launch_product(fc3_f8(c, n), IN_F8_E8, OUT_F32, st)); plan_note("fc3_e4m3"); break;
       case Fc3::F32:  HIP_TRY(c, launch_fc_gemm(c->h1, c->fc2w, c->fc2b, c->h2, n, FC2, FC1, 1, st)); break;
       case Fc3::Gemv: HIP_TRY(c, launch_fc_gemv(c->h1, c->fc2w, c->fc2b, c->h2, n, FC2, FC1, 1, st)); break;
       case Fc3::Bf16: HIP_TRY(c, launch_fc_gemm_bf16(c->h1, c->fc2w_bf16, c->fc2b, c->h2, 0, n, FC2, FC1, 1, st)); break;
@@ -926,7 +1017,7 @@ void dce_destroy(dce_ctx* c)
     if (c->xfer_stream) { hipStreamSynchronize(c->xfer_stream); hipStreamDestroy(c->xfer_stream); }
     for (auto& slot : c->ring_ev) for (auto e : slot) if (e) hipEventDestroy(e);
     dev_free(c->d_weights); dev_free(c->feat); dev_free(c->feat3); dev_free(c->h1); dev_free(c->h2); dev_free(c->part);
-    dev_free(c->feat_scale); dev_free(c->h1h); dev_free(c->h1_scale); dev_free(c->d_guard); dev_free(c->fc1w_x3_own); dev_free(c->h1p); dev_free(c->d_in); dev_free(c->d_logits); dev_free(c->d_pred); dev_free(c->d_contacts); dev_free(c->d_packed);
+    dev_free(c->feat_scale); dev_free(c->h1h); dev_free(c->h1_scale); dev_free(c->d_guard); dev_free(c->fc1w_x3_own); dev_free(c->h1p); dev_free(c->f8); dev_free(c->d_in); dev_free(c->d_logits); dev_free(c->d_pred); dev_free(c->d_contacts); dev_free(c->d_packed);
     if (c->online_exec) hipGraphExecDestroy(c->online_exec);
     if (c->online_graph) hipGraphDestroy(c->online_graph);
     dev_free(c->d_ring); dev_free(c->d_online_state);
@@ -975,8 +1066,9 @@ int dce_load_weight(dce_ctx* c, const char* key, const float* host, const int64_
 int dce_finalize_weights(dce_ctx* c, int precision)
 {
     if (!c) return DCE_ERR_ARG;
-    if (precision != DCE_FP32 && precision != DCE_BF16_FC && precision != DCE_FP32_SPLIT && precision != DCE_FP32_F16X2)
-        return fail(c, DCE_ERR_ARG, "unknown precision %d (0 = fp32, 1 = bf16 FC, 2 = fp32 on three-term bf16 operands, 3 = fp32 tolerance on two-term fp16 operands)", precision);
+    if (precision != DCE_FP32 && precision != DCE_BF16_FC && precision != DCE_FP32_SPLIT && precision != DCE_FP32_F16X2 && precision != DCE_FP8_FC)
+        return fail(c, DCE_ERR_ARG, "unknown precision %d (0 = fp32, 1 = bf16 FC, 2 = fp32 on three-term bf16 operands, 3 = fp32 tolerance on two-term fp16 operands, 4 = 8-bit FC)", precision);
+    const bool bf16_conv = precision == DCE_BF16_FC || precision == DCE_FP8_FC;      // conv stacks that write bf16 features
     for (int k = 0; k < 14; ++k)
         if (!c->have[k]) return fail(c, DCE_ERR_STATE, "missing state_dict key '%s'", kKeys[k].name);
     c->split_alias = false;
@@ -1029,7 +1121,7 @@ int dce_finalize_weights(dce_ctx* c, int precision)
         off_mb1 = reserve(latmb_pack_floats(FC1, FEAT)); latmb_pack_host(c->host_w[8].data(), FC1, FEAT, img.data() + off_mb1, 128);
         off_mb2 = reserve(latmb_pack_floats(FC2, FC1));  latmb_pack_host(c->host_w[10].data(), FC2, FC1, img.data() + off_mb2, 0);
     }
-    const bool want_cx = precision == DCE_FP32_SPLIT || (precision == DCE_BF16_FC && c->tuning.x3_conv);
+    const bool want_cx = precision == DCE_FP32_SPLIT || (bf16_conv && c->tuning.x3_conv);
     const bool want_pair = (want_cx && (c->tuning.x3_pair || c->tuning.x3_permk)) || precision == DCE_FP32_F16X2;      // fc.0's weights once more, K axis in the conv kernels' feature order t' * 128 + c
     std::vector<float> w1p;
     if (want_pair) { w1p.resize(c->host_w[8].size()); fc_perm_k_host(c->host_w[8].data(), FC1, w1p.data()); }
@@ -1076,7 +1168,7 @@ int dce_finalize_weights(dce_ctx* c, int precision)
     ConvPackH2 h2pk{};
     int h2_fc_sw = 0, h2_fc2_sw = 0, h2_eW = 0, h2_eB = 0;
     bool h2_bad = false;
-    const bool h2_conv_only = precision == DCE_BF16_FC && c->tuning.bf16_conv_h2 && want_pair;      // DCE_BF16_FC with its conv stack on conv_h2.hip: the conv packs alone
+    const bool h2_conv_only = bf16_conv && c->tuning.bf16_conv_h2 && want_pair;      // DCE_BF16_FC / DCE_FP8_FC with its conv stack on conv_h2.hip: the conv packs alone
     if (precision == DCE_FP32_F16X2 || h2_conv_only) {
         for (int l = 0; l < 4 && !h2_bad; ++l) {
             const auto& w = c->host_w[2 * l]; const auto& b = c->host_w[2 * l + 1];
@@ -1156,6 +1248,8 @@ int dce_finalize_weights(dce_ctx* c, int precision)
     c->fc1_sw = h2_fc_sw;
     c->fc2w_h2 = precision == DCE_FP32_F16X2 && !h2_bad && c->tuning.h2_fc3 ? reinterpret_cast<const unsigned short*>(c->d_weights + off_h2fc2) : nullptr;
     c->fc2_sw = h2_fc2_sw; c->fc1_eW = h2_eW; c->fc1_eB = h2_eB;
+    c->fc1w_f8 = c->fc1s_f8 = c->fc1w_f8p = c->fc1s_f8p = c->fc2w_f8 = c->fc2s_f8 = nullptr;
+    if (precision == DCE_FP8_FC) { const int rc = quantize_weights_f8(c, w1p); if (rc) return rc; }
     c->precision = precision;
     c->guard = dce_ctx::SplitGuard{};
 #if DCE_EXPERIMENTS
@@ -1272,6 +1366,8 @@ int dce_forward_taps(dce_ctx* c, const float* windows, int64_t n, int on_device,
     DEVICE_GUARD(c);
     if (n <= 0 || n > c->max_batch || !windows)
         return fail(c, DCE_ERR_ARG, "dce_forward_taps: need 0 < n <= max_batch (%lld)", (long long)c->max_batch);
+    if (c->precision == DCE_FP8_FC && (feat || h1))
+        return fail(c, DCE_ERR_STATE, "dce_forward_taps: features and h1 are e4m3 with scales in DCE_FP8_FC: h2 and logits only");
     const float* dsrc = windows;
     float* dl = logits;
     if (!on_device) {
@@ -1314,8 +1410,8 @@ int dce_conv_layer_taps(dce_ctx* c, const float* windows, int64_t n, int kernel,
         return fail(c, DCE_ERR_STATE, "dce_conv_layer_taps: kernel 7 (conv_x3) needs a context finalised with DCE_FP32_SPLIT");
     if (kernel == 8 && (c->precision != DCE_FP32_F16X2 || c->h2_refused))
         return fail(c, DCE_ERR_STATE, "dce_conv_layer_taps: kernel 8 (conv_h2) needs a context finalised with DCE_FP32_F16X2 (and a finite checkpoint)");
-    if (c->precision == DCE_BF16_FC)
-        return fail(c, DCE_ERR_STATE, "dce_conv_layer_taps: not available in DCE_BF16_FC (its conv stack is the fp32 / three-term one: tap a DCE_FP32 or DCE_FP32_SPLIT context)");
+    if (c->precision == DCE_BF16_FC || c->precision == DCE_FP8_FC)
+        return fail(c, DCE_ERR_STATE, "dce_conv_layer_taps: not available in DCE_BF16_FC / DCE_FP8_FC (its conv stack is the fp32 / three-term one: tap a DCE_FP32 or DCE_FP32_SPLIT context)");
     TuningScope tuning_scope(&c->tuning);                 // the launchers below read this context's switches, not the process defaults
     // host pointers only (a test hook): stage the windows, run ONE named kernel family with its taps on, copy everything out
     const size_t in_f = (size_t)n * WIN * CH;
@@ -1338,6 +1434,26 @@ int dce_conv_layer_taps(dce_ctx* c, const float* windows, int64_t n, int kernel,
     for (int i = 0; i < 5; ++i) HIP_TRY(c, hipMemcpyAsync(outs[i], srcs[i], sz[i] * sizeof(float), hipMemcpyDeviceToHost, c->stream));
     HIP_TRY(c, hipMemcpyAsync(feat, c->feat, (size_t)n * FEAT * sizeof(float), hipMemcpyDeviceToHost, c->stream));
     HIP_TRY(c, hipStreamSynchronize(c->stream));
+    return DCE_OK;
+}
+
+int dce_features(dce_ctx* c, const float* src, int64_t n, int zscore, void* feat)
+{
+    int rc = check_ready_quiet(c);
+    if (rc) return rc;
+    DEVICE_GUARD(c);
+    if (c->precision != DCE_BF16_FC && c->precision != DCE_FP8_FC) return fail(c, DCE_ERR_STATE, "dce_features: bf16 features need a context finalized with DCE_BF16_FC or DCE_FP8_FC");
+    if (!c->pkx3.w[0]) return fail(c, DCE_ERR_STATE, "dce_features: the option x3_conv=0 leaves out the conv kernels it runs");
+    if (n < 0 || (n && (!src || !feat)) || (reinterpret_cast<uintptr_t>(feat) & 15)) return fail(c, DCE_ERR_ARG, "dce_features: need n >= 0 and 16-byte aligned features");
+    TuningScope tuning_scope(&c->tuning);
+    struct PlanScope { explicit PlanScope(std::vector<const char*>* p) { p->clear(); t_plan = p; } ~PlanScope() { t_plan = nullptr; } } plan_scope(&c->plan);
+    const int64_t row = zscore ? CH : (int64_t)WIN * CH;
+    for (int64_t i = 0; i < n; i += c->max_batch) {                   // (as run_all cuts a call: a launch's size decides its kernel)
+        const int64_t m = n - i < c->max_batch ? n - i : c->max_batch;
+        unsigned short* out = static_cast<unsigned short*>(feat) + (size_t)i * FEAT;
+        if (m >= plan_threshold(c->tuning, T_BF16H2) && c->tuning.bf16_conv_h2 && c->pkh2.w[0]) HIP_TRY(c, launch_conv_h2_bf16(src + i * row, zscore, m, c->pkh2, out, c->stream));
+        else HIP_TRY(c, launch_conv_x3_bf16(src + i * row, zscore, m, c->pkx3, out, c->stream, 1, DCE_EXPERIMENTS ? c->tuning.x3_bf16_terms : 2, nullptr));
+    }
     return DCE_OK;
 }
 

@@ -49,6 +49,9 @@ struct dce_ctx {
     const void *fc1w_bf16 = nullptr, *fc2w_bf16 = nullptr;   // DCE_BF16_FC only
     const void* fc1w_bf16p = nullptr;                        // ... fc.0 with its K axis in conv_x3p.hip's feature order (t' * 128 + c)
 
+    unsigned char* f8 = nullptr;                             // DCE_FP8_FC: one allocation with what follows: e4m3 weights of fc.0 (both feature orders) and fc.3, e8m0 scales
+    const unsigned char *fc1w_f8 = nullptr, *fc1s_f8 = nullptr, *fc1w_f8p = nullptr, *fc1s_f8p = nullptr, *fc2w_f8 = nullptr, *fc2s_f8 = nullptr;
+
     float *feat = nullptr, *h1 = nullptr, *h2 = nullptr;   // scratch, max_batch rows each
     unsigned short* feat3 = nullptr;                        // DCE_FP32_SPLIT: the features as three bf16 planes [3][n][4736]
     dce::ConvPackX3 pkx3{};                                      // ... and the conv weights, packed per lane (conv_x3.hip)

@@ -41,9 +41,9 @@ def main(argv=None):
                         default=os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "config",
                                              "inference_one_seq_params.yaml"))
     parser.add_argument("--fused", action="store_true", help="one fused pass instead of the batch loop")
-    parser.add_argument("--precision", default=None, choices=["fp32", "bf16_fc", "fp32_split", "fp32_f16x2"],
+    parser.add_argument("--precision", default=None, choices=["fp32", "bf16_fc", "fp32_split", "fp32_f16x2", "fp8_fc"],
                         help="arithmetic of the library (default fp32 = the reference's; the YAML may carry a `precision` key too): "
-                             "bf16_fc = bf16 operands on fc.0 / fc.3; fp32_split = fp32 results on the bf16 matrix pipe (DESIGN.md 4.1x / 4.2x); "
+                             "bf16_fc = bf16 operands on fc.0 / fc.3; fp8_fc = 8-bit operands there; fp32_split = fp32 results on the bf16 matrix pipe (DESIGN.md 4.1x / 4.2x); "
                              "fp32_f16x2 = the fp32 tolerance from two fp16 terms per operand with per-window scales (DESIGN.md 4.6)")
     parser.add_argument("--latency", action="store_true",
                         help="the library's latency mode (fp32; option latency=1, a `latency: true` key in the YAML does the same): every batch of up to 32 windows "

@@ -82,7 +82,7 @@ typedef enum dce_precision {
                                   product, behind a RANGE GUARD (static per-layer bounds at dce_finalize_weights, a per-window check in the conv
                                   kernel and a gated DCE_FP32 kernel sequence behind every guarded launch; dce_split_guard_info) -- lives on in the
                                   experiments build (libdce_experiments.so: csrc/conv_x3.hip, csrc/fc_gemm_x3.hip), with its tests */
-    DCE_FP32_F16X2      = 3    /* fp32-TOLERANCE results with the conv stack (from 128 windows per launch), fc.0 and fc.3 (from 1281; below
+    DCE_FP32_F16X2      = 3,   /* fp32-TOLERANCE results with the conv stack (from 128 windows per launch), fc.0 and fc.3 (from 1281; below
                                   that the DCE_FP32 kernels) on the fp16 matrix pipe: every operand is scaled by a power of two and
                                   enters as TWO fp16 terms (11 + 11 significand bits), three MFMAs per product, fp32 accumulate
                                   (csrc/conv_h2.hip, csrc/fc_gemm_h2.hip; 2.5 x DCE_FP32's throughput at 4096 windows).  Not fp32 operands -- 22 of their 24 bits -- but the same contract
@@ -91,6 +91,12 @@ typedef enum dce_precision {
                                   for the activations, chosen by the kernel from the layer's largest output -- keep every operand inside
                                   fp16's range whatever the input: no range guard, no fallback, and a window's result depends on that
                                   window alone.  A checkpoint with a non-finite weight runs the DCE_FP32 kernels.  Opt-in */
+    DCE_FP8_FC          = 4    /* DCE_BF16_FC with fc.0 / fc.3 in 8 bits: the bf16 features, h1 and the weights of both layers are e4m3 with a power of two for
+                                  every 128 values (dce_quantize's rule; weights: 128 x 128), sums fp32, h2 and fc.6 fp32 (csrc/block_quant.hip,
+                                  csrc/block_gemm.hip).  CONTRACT: logits as near an fp32 / fp64 evaluation as 4-bit significands on fc.0 and fc.3 leave
+                                  them (the sum of every rounding's largest effect; tests/test_fp8_bank_gpu.py works it out): check a checkpoint's accuracy
+                                  before serving it so.  Which kernels run, and with them the last bits, goes by the size of the launch.  A non-finite weight makes NaN of what it touches.  The taps hand out
+                                  h2 and the logits alone.  Opt-in */
 } dce_precision;
 /* Batch-size regimes.  DCE_FP32 gives a window the same bits whatever the size of the call it arrives in (one fixed summation tree in
  * every kernel family; latency=1 contexts: whole calls of up to 32 windows take one-kernel forms with another summation order, see below).  The two
@@ -337,6 +343,11 @@ int  dce_debug_latency_trace(dce_ctx* ctx, unsigned long long stamps[16]);
  * placement (the placement of `ctx`; a plain hipMalloc for a context without the option).  tests/test_guard_alloc_gpu.py, tools/guard_stress.py. */
 int  dce_debug_alloc(dce_ctx* ctx, size_t bytes, void** device_ptr);
 int  dce_debug_free(dce_ctx* ctx, void* device_ptr);
+
+/* The conv stack alone (src/contact_cnn.py:60-64 up to the flatten), for FC layers of the caller's own (dce_matmul): windows (n,150,54) already z-scored,
+ * or raw rows (n + 149, 54) with zscore != 0 -> feat (n, 4736) bf16, value (t, c) of a window at t * 128 + c, t < 37, c < 128 (the reference flattens to
+ * c * 37 + t: permute fc.0's columns).  DEVICE pointers; contexts finalized with DCE_BF16_FC or DCE_FP8_FC; asynchronous on the ctx stream. */
+int  dce_features(dce_ctx* ctx, const float* src, int64_t n, int zscore, void* feat);
 
 /* ---- The matrix products of the FC layers as operators of their own -------------------------------------------------------------------------
  * Not in the reference, whose FC layers are torch.nn.Linear (src/contact_cnn.py:48-57): the 8-bit form of such a layer, and one layer of many
