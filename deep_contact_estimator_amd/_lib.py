@@ -11,6 +11,8 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DCE_LIB") or os.path.join(_HERE, "libdce.so")   # DCE_LIB: A/B builds
 
+ENTRIES_PATH = os.path.join(_HERE, "_entries.so")                   # ops.py's extension module (csrc/torch_entries.cpp)
+
 # every symbol include/dce.h declares: (name, restype, argtypes)
 _i64p = C.POINTER(C.c_int64)
 SYMBOLS = {

@@ -50,6 +50,36 @@ def built_hash(lib: str = LIB) -> str | None:
         return None
 
 
+ENTRIES, ENTRIES_SOURCE = os.path.join(HERE, "_entries.so"), "torch_entries.cpp"
+
+
+def build_entries(force: bool = False) -> str | None:
+    """_entries.so: ops.py's entries on torch tensors (csrc/torch_entries.cpp), a CPython extension module compiled against the installed torch; None
+    without torch (the package works on numpy arrays without it)."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    import hashlib
+    import sysconfig
+    h = hashlib.sha256(torch.__version__.encode())
+    for path in (os.path.join(CSRC, ENTRIES_SOURCE), os.path.join(HERE, "..", "include", "dce.h")):
+        h.update(open(path, "rb").read())
+    if not force and os.path.exists(ENTRIES) and built_hash(ENTRIES) == h.hexdigest():
+        return ENTRIES
+    t = os.path.dirname(torch.__file__)
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", os.path.join(t, "include"), "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, ENTRIES_SOURCE), "-o", ENTRIES + ".tmp",
+           "-L", os.path.join(t, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("compile failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+    os.replace(ENTRIES + ".tmp", ENTRIES)
+    with open(ENTRIES + ".srchash", "w") as f:
+        f.write(h.hexdigest() + "\n")
+    return ENTRIES
+
+
 def file_flags(source: str) -> list[str]:
     """Flags of one translation unit beside CFLAGS."""
     return ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if source in NO_PACKED_FP32 else []
@@ -98,6 +128,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     (PyTorch wheels bundle their own libamdhip64/libhsa-runtime64; a second copy from
     /opt/rocm in the same process cannot open the device).  _lib.load() puts the right runtime
     in the global symbol scope first."""
+    build_entries(force)
     if not force and not stale():
         return LIB
     os.makedirs(OBJDIR, exist_ok=True)

@@ -7,6 +7,8 @@ import struct
 import pytest
 
 torch = pytest.importorskip("torch")
+QUANTIZE = struct.Struct("=QqqQqqQqqqqiiii")                       # the descriptors as a C caller packs them
+MATMUL = struct.Struct("=QqQqQqqQqqQqQqQqQQqqqqiiiiii")
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -28,30 +30,27 @@ def _fields(name):
     return found
 
 
-@pytest.mark.parametrize("name, packed", [("dce_quantize_desc", "_QUANTIZE"), ("dce_matmul_desc", "_MATMUL")])
+@pytest.mark.parametrize("name, packed", [("dce_quantize_desc", QUANTIZE), ("dce_matmul_desc", MATMUL)])
 def test_descriptors_match_the_header(name, packed):
-    from deep_contact_estimator_amd import ops
     fields = _fields(name)
     codes = "".join("Q" if k.endswith("*") else "q" if k == "int64_t" else "i" for k, _ in fields)
-    assert getattr(ops, packed).format == "=" + codes
+    assert packed.format == "=" + codes
     kinds = {"Q": C.c_void_p, "q": C.c_int64, "i": C.c_int32}
     struct_type = type(name, (C.Structure,), {"_fields_": [(f, kinds[c]) for (_, f), c in zip(fields, codes)]})
-    assert C.sizeof(struct_type) == getattr(ops, packed).size            # no padding between the fields
+    assert C.sizeof(struct_type) == packed.size            # no padding between the fields
 
 
 def _quantize(**kw):
     d = dict(x=4096, ldx=256, x_batch=0, q=8192, ldq=256, q_batch=0, scale=1024, ld_scale=4, batch=1, rows=4, k=256, x_type=0, scale_type=0, block_rows=1, reserved=0)
     d.update(kw)
-    from deep_contact_estimator_amd import ops
-    return ops._QUANTIZE.pack(*d.values())
+    return QUANTIZE.pack(*d.values())
 
 
 def _matmul(**kw):
     d = dict(a=4096, lda=256, a_scale=4096, ld_a_scale=4, b=4096, ldb=256, b_group=0, b_scale=4096, ld_b_scale=2, b_scale_group=0, bias=0, bias_group=0,
              y=8192, ldy=64, y_scale=0, ld_y_scale=0, offsets=0, index=0, a_rows=4, m=4, n=64, k=256, groups=1, in_type=2, scale_type=0, out_type=0, relu=0, reserved=0)
     d.update(kw)
-    from deep_contact_estimator_amd import ops
-    return ops._MATMUL.pack(*d.values())
+    return MATMUL.pack(*d.values())
 
 
 @pytest.mark.parametrize("kw, word", [
