@@ -11,7 +11,9 @@
 // The weights are the instruction's FIRST operand: a lane then holds four neighbouring columns of one row of y (one activation scale a lane, vector
 // stores).  Lane l: row l & 15 of either operand, chunks l >> 4 and (l >> 4) + 4.
 #include "block_ops.h"
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace dce {
 
@@ -71,7 +73,7 @@ __device__ __forceinline__ long long source_row(const ProductArgs& p, int j, int
 __device__ __forceinline__ int slot_of(int r, int c) { return r * KROW + ((c ^ ((r >> 1) & 7)) * 16); }
 __device__ __forceinline__ i32x4 chunk(const char* lds, int r, int c) { return *reinterpret_cast<const i32x4*>(lds + slot_of(r, c)); }
 
-// 32 e4m3 values -> fp16, without error
+// 16 e4m3 values -> fp16, without error
 __device__ __forceinline__ void to_f16(i32x4 v, f16x8& lo, f16x8& hi)
 {
     f16x2 h[8];
@@ -83,43 +85,68 @@ __device__ __forceinline__ void to_f16(i32x4 v, f16x8& lo, f16x8& hi)
     lo = __builtin_shufflevector(__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3), __builtin_shufflevector(h[2], h[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
     hi = __builtin_shufflevector(__builtin_shufflevector(h[4], h[5], 0, 1, 2, 3), __builtin_shufflevector(h[6], h[7], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
+// ... times the power of two of an e8m0 byte -> bf16, without error (bf16 has fp32's range)
+__device__ __forceinline__ void to_bf16x16(i32x4 v, unsigned byte, bf16x8& lo, bf16x8& hi)
+{
+    const float s = __uint_as_float(byte << 23);                              // (the instruction takes the exponent alone)
+    bf16x2 h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], s, false);
+        h[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], s, true);
+    }
+    lo = __builtin_shufflevector(__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3), __builtin_shufflevector(h[2], h[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+    hi = __builtin_shufflevector(__builtin_shufflevector(h[4], h[5], 0, 1, 2, 3), __builtin_shufflevector(h[6], h[7], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
-// One row's 32 values of a step as a lane holds them for the matrix instruction.  EXACT: e4m3 as fp16 (see mac)
+// One row's 128 bytes of a step as a lane holds its quarter of them for the matrix instruction.  EXACT: e4m3 in 16 bits (see mfma_row); `scale`: the
+// row's, or the weights', e8m0 byte
 template <int IN, bool EXACT> struct Frag {
     i32x4 c0, c1;
-    __device__ __forceinline__ void set(i32x4 a, i32x4 b) { c0 = a; c1 = b; }
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b, unsigned) { c0 = a; c1 = b; }
 };
-template <int IN> struct Frag<IN, true> {
+template <> struct Frag<IN_F8_F32, true> {
     f16x8 h[4];
-    __device__ __forceinline__ void set(i32x4 a, i32x4 b) { to_f16(a, h[0], h[1]); to_f16(b, h[2], h[3]); }
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b, unsigned) { to_f16(a, h[0], h[1]); to_f16(b, h[2], h[3]); }
 };
-template <> struct Frag<IN_BF16, true> : Frag<IN_BF16, false> {};
+template <> struct Frag<IN_F8_E8, true> {
+    bf16x8 h[4];
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b, unsigned scale) { to_bf16x16(a, scale, h[0], h[1]); to_bf16x16(b, scale, h[2], h[3]); }
+};
 
-// The scales of a step for a lane's row of x and a block of columns.  fp32: their product.  e8m0: the two bytes for the matrix instruction, or (EXACT) the
-// sum of the exponents; a byte of 255 is NaN there too.
+// The scales of a step for a lane's row of x and a block of columns.  fp32: their product.  e8m0: the two bytes for the 8-bit matrix instruction, whose
+// byte 255 is NaN; where the fragments took them (EXACT) `bad` remembers that there was one.
 template <int IN, bool EXACT> struct Scale {
-    float s, start; int e, ew, ex;
-    // of the weights' block and of x's row: fp32 numbers, or bytes
-    __device__ __forceinline__ void set(unsigned w, unsigned x)
+    float s; int ew, ex;
+    __device__ __forceinline__ void set(unsigned w, unsigned x, unsigned& bad)
     {
         if (IN == IN_F8_F32) s = __uint_as_float(w) * __uint_as_float(x);
-        else if (EXACT) { e = (int)(w + x) - 254; start = w == 255 || x == 255 ? __builtin_nanf("") : 0.f; }
+        else if (EXACT) bad |= w == 255 || x == 255;
         else { ew = (int)w; ex = (int)x; }
     }
 };
+template <int IN, bool EXACT, int NT>
+__device__ __forceinline__ void spoil(f32x4 (&acc)[NT], unsigned bad)
+{
+    if constexpr (IN == IN_F8_E8 && EXACT)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = bad ? __builtin_nanf("") : acc[j][i];
+}
 
 // acc += the product of a block of 16 x 16 over one step of K.
 //
 // The 8-bit matrix instruction lines the eight products of a group up with the largest of them and keeps 13 bits below its leading one (measured: of
 // 65536 + 8 everything, of 65536 + 4 nothing is left of the second; between groups sums are fp32): on random operands 1.5e-5 of the result, a hundredth
 // of the rounding to bf16 (1.7e-3) and less still of that to e4m3, so results in those types take it.  fp32 results would be a hundred times worse
-// than their type: they take the operands as fp16 (every e4m3 number is one) through the fp16 instruction, at half the rate, whose sums of 32 products
-// are good to 1e-8.
+// than their type: their operands go through the 16-bit instructions, at half the rate, whose sums of 32 products are good to 1e-8 -- with e8m0 scales
+// as bf16 with the scale in it, with fp32 scales as fp16 (every e4m3 number is one).
 //
 // One row of blocks at a time: instructions that add to the same sums are as far apart as the row is long (a dependent one waits for its predecessor).
 // Where the matrix instruction can apply the scales (or there are none) it adds to `acc`; otherwise the block's sums go to `part` and fold_row brings
 // them home -- behind the next row's matrix instructions, which hide it.
-template <int IN, bool EXACT> constexpr bool FOLDS = IN != IN_BF16 && (EXACT || IN == IN_F8_F32);
+template <int IN, bool EXACT> constexpr bool FOLDS = IN == IN_F8_F32;
 
 template <int IN, bool EXACT, int NT>
 __device__ __forceinline__ void mfma_row(f32x4 (&acc)[NT], f32x4 (&part)[NT], const Frag<IN, EXACT> (&w)[NT], const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
@@ -130,11 +157,13 @@ __device__ __forceinline__ void mfma_row(f32x4 (&acc)[NT], f32x4 (&part)[NT], co
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[j].c1), __builtin_bit_cast(bf16x8, x.c1), acc[j], 0, 0, 0);
     } else if constexpr (EXACT) {
-        const float z = IN == IN_F8_E8 ? sc.start : 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j].h[k], x.h[k], k ? part[j] : f32x4{z, z, z, z}, 0, 0, 0);
+            for (int j = 0; j < NT; ++j) {
+                if constexpr (IN == IN_F8_E8) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j].h[k], x.h[k], acc[j], 0, 0, 0);
+                else part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j].h[k], x.h[k], k ? part[j] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            }
     } else {
         const i32x8 xv = __builtin_shufflevector(x.c0, x.c1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
@@ -152,7 +181,7 @@ __device__ __forceinline__ void fold_row(f32x4 (&acc)[NT], const f32x4 (&part)[N
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = IN == IN_F8_E8 ? acc[j][i] + ldexpf(part[j][i], sc.e) : fmaf(part[j][i], sc.s, acc[j][i]);
+            for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[j][i], sc.s, acc[j][i]);
 }
 template <int IN, bool EXACT, int NT>
 __device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> (&w)[NT], const Frag<IN, EXACT>& x, const Scale<IN, EXACT>& sc)
@@ -163,19 +192,6 @@ __device__ __forceinline__ void mac_row(f32x4 (&acc)[NT], const Frag<IN, EXACT> 
 }
 
 __device__ __forceinline__ unsigned short to_bf16(float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
-
-__device__ __forceinline__ f32x4 finish(const ProductArgs& p, f32x4 v, const float* bias, int c)
-{
-    if (bias) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (c + i < p.n) v[i] += bias[c + i];
-    }
-    if (p.relu) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];          // (NaN stays)
-    }
-    return v;
-}
 
 // four neighbouring columns c .. of row j
 template <int OUT>
@@ -208,9 +224,10 @@ __device__ __forceinline__ bool wide_stores(const ProductArgs& p, int bytes)
 
 }  // namespace
 
-// ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave.  A step's panels and scales
-//      come by LDS-DMA into a ring of NBUF buffers, NBUF - 1 steps ahead, fragments from there into registers a step ahead of their instructions; one
-//      barrier a step.
+// ---- the kernel for operands whose rows start at multiples of 16 bytes: BM x BN a workgroup, MT x NT blocks of 16 x 16 a wave, the steps of K dealt
+//      out in turn to KG groups of four waves, each with panels of its own, that add up their sums at the end (group 0's first).  A step's panels and
+//      scales come by LDS-DMA into a ring of NBUF buffers, fragments from there into registers a step ahead of their instructions; one barrier for KG
+//      steps.  The requests are what bounds it (a CU takes one of 1 KB in 16 cycles), then the barrier: two groups share that.
 // 64 lanes x 16 bytes from `from` + the lanes' offsets to LDS at `lds` (+ lane * 16)
 __device__ __forceinline__ void dma16s(const char* from, unsigned at, unsigned lds)
 {
@@ -228,13 +245,13 @@ __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(
 
 template <int N> __device__ __forceinline__ void wait_all_but() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
-template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Ring {
-    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;   // waves along the rows / the columns; blocks of 16 a wave
-    static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
+template <int WM_, int WN_, int MT_, int NT_, int NBUF_, int KG_> struct Ring {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_, KG = KG_;   // waves along the rows / the columns; blocks of 16 a wave
+    static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES * KG;
     static constexpr int PANELS = (BM + BN) * KROW, PIECES = PANELS / 1024 / WAVES;   // a piece: eight rows, one instruction
-    static constexpr int SLOT = ((BM + 63) / 64 * 64 + 64) * 4, BUF = PANELS + SLOT;  // the rows' scales, the columns': a word each
-    static constexpr int LDS = NBUF * BUF;
-    static_assert(PANELS % (1024 * WAVES) == 0 && BM % 8 == 0 && BN == BLK && LDS <= 160 * 1024 && (BM + 63) / 64 <= WAVES, "tile");
+    static constexpr int SA = (BM + 63) / 64, SLOT = (SA + 1) * 256, BUF = PANELS + SLOT;  // waves that bring the rows' scales; a word a row, then the columns'
+    static constexpr int LDS = KG * NBUF * BUF;
+    static_assert(PANELS % (1024 * WAVES) == 0 && BM % 8 == 0 && BN == BLK && LDS <= 160 * 1024 && SA < WAVES && WAVES == 4, "tile");
 };
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
@@ -333,14 +350,17 @@ template <int IN, int OUT, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs p)
 {
     constexpr bool EXACT = OUT == OUT_F32;
-    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, NBUF = T::NBUF, PS = IN != IN_BF16 ? 2 : 0;
+    constexpr int BM = T::BM, MT = T::MT, NT = T::NT, NBUF = T::NBUF, KG = T::KG, PS = IN != IN_BF16;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     Place place;
     if (!find_tile(p, BM, place)) return;
     const int g = place.g, first = place.first, end = place.end, n0 = place.tn * T::BN;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % T::WAVES, kg = all / T::WAVES, r = lane & 15, q = lane >> 4;
     const int wm = (wave / T::WN) * MT * 16, wn = (wave % T::WN) * NT * 16;
-    const int steps = (p.kbytes + KROW - 1) / KROW;
+    const int total = (p.kbytes + KROW - 1) / KROW, rounds = (total + KG - 1) / KG;   // this group's steps: kg, kg + KG, ..; a round: one of every group
+    const int steps = kg < total ? (total - kg + KG - 1) / KG : 0;
+    const int tail = p.kbytes % KROW;                                         // bytes of the last step, where K ends inside it
+    const bool mine = tail && (total - 1) % KG == kg;                         // ... and it is this group's
 
     unsigned from[T::PIECES];                                                 // from the step's column of a, of the group's b
 #pragma unroll
@@ -352,66 +372,78 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
         asm volatile("" : "+v"(row));                                         // (a product and a sum of 32 bits: not the instruction whose result fills two registers)
         from[i] = row + col;
     }
-    // the scales of 64 rows (several waves may bring the same ones) and of the column block (all waves)
+    // scales: waves 0 .. SA - 1 bring those of 64 rows each, the last wave that of the columns
     constexpr int SZ = IN == IN_F8_F32 ? 4 : 1;
-    const int s_row = wave % ((BM + 63) / 64) * 64;
-    const char *ka = p.a, *kb = p.b + g * p.b_group, *sa = static_cast<const char*>(p.sa), *sb = nullptr;
-    unsigned sa_at = 0, none = 0;
-    if (PS) {
-        const long long s = s_row + lane < BM ? source_row(p, first + s_row + lane, end) : -1;
-        sa_at = (unsigned)(s < 0 ? 0 : s) * SZ;
-        sb = static_cast<const char*>(p.sb) + (g * p.sb_group + (long long)place.tn * p.sb_row) * SZ;
-        asm volatile("" : "+v"(none));
+    const bool rows_too = PS && wave < T::SA, cols_too = PS && wave == T::WAVES - 1;
+    const char *ka = p.a + kg * KROW, *kb = p.b + g * p.b_group + kg * KROW, *ks = nullptr;
+    long long s_step = 0;
+    unsigned s_at = 0;
+    if (rows_too) {
+        const long long s = wave * 64 + lane < BM ? source_row(p, first + wave * 64 + lane, end) : -1;
+        s_at = (unsigned)(s < 0 ? 0 : s) * SZ;
+        ks = static_cast<const char*>(p.sa) + kg * p.sa_block * SZ;
+        s_step = KG * p.sa_block * SZ;
+    } else if (cols_too) {
+        ks = static_cast<const char*>(p.sb) + (g * p.sb_group + (long long)place.tn * p.sb_row + kg) * SZ;
+        s_step = KG * SZ;
     }
-    const unsigned lds0 = lds_addr(smem);
+    char* const ring = smem + kg * NBUF * T::BUF;
+    const unsigned lds0 = lds_addr(ring);
     int to = 0;                                                               // the buffer of the next step asked for
-    const int tail = p.kbytes % KROW;                                         // bytes of the last step, where K ends inside it
     auto tail_col = [&](int i) { const int lr = (i * T::WAVES + wave) * 8 + (lane >> 3); return ((lane & 7) ^ ((lr >> 1) & 7)) * 16; };
-    // pieces lo .. hi - 1 of step s (the last ones: its scales)
-    constexpr int ALL = T::PIECES + PS;
+    // pieces lo .. hi - 1 of this group's step s (behind the last one: its scales)
     auto bring = [&](int s, int lo, int hi) {
         const unsigned at = lds0 + to * T::BUF;
-        if (lo == 0 && tail && s == steps - 1) {                                         // chunks behind the end: any that are there, made zeros below
+        if (lo == 0 && mine && s == steps - 1) {                              // chunks behind the end: any that are there, made zeros below
 #pragma unroll
             for (int i = 0; i < T::PIECES; ++i) if (tail_col(i) >= tail) from[i] -= tail_col(i);
         }
 #pragma unroll
         for (int i = 0; i < T::PIECES; ++i) if (i >= lo && i < hi) dma16s((i * T::WAVES + wave) * 8 < BM ? ka : kb, from[i], at + (i * T::WAVES + wave) * 1024);
-        if (hi < ALL) return;
-        ka += KROW;
-        kb += KROW;
-        if constexpr (PS != 0) {
-            if constexpr (SZ == 4) { dma4s(sa, sa_at, at + T::PANELS + s_row * 4); dma4s(sb, none, at + T::PANELS + T::SLOT - 256); }
-            else { dma1s(sa, sa_at, at + T::PANELS + s_row * 4); dma1s(sb, none, at + T::PANELS + T::SLOT - 256); }
-            sa += p.sa_block * SZ;
-            sb += SZ;
-        }
+        if (hi < T::PIECES) return;
+        ka += KG * KROW;
+        kb += KG * KROW;
+        if constexpr (PS)
+            if (rows_too || cols_too) {
+                const unsigned slot = at + T::PANELS + (cols_too ? T::SA : wave) * 256;
+                if constexpr (SZ == 4) dma4s(ks, s_at, slot);
+                else dma1s(ks, s_at, slot);
+                ks += s_step;
+            }
         to = to == NBUF - 1 ? 0 : to + 1;
+    };
+    // all of this wave's requests but those of the last `ahead` steps have landed
+    auto landed = [&](auto ahead) {
+        constexpr int N = decltype(ahead)::value;
+        if (rows_too || cols_too) wait_all_but<N * (T::PIECES + 1)>();
+        else wait_all_but<N * T::PIECES>();
     };
 
     f32x4 acc[MT][NT];
+    unsigned bad[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
+        bad[i] = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
-    for (int s = 0; s < NBUF; ++s) if (s < steps) bring(s, 0, ALL);
+    for (int s = 0; s < NBUF; ++s) if (s < steps) bring(s, 0, T::PIECES);
     int buf = 0;
     struct Step { i32x4 w0[NT], w1[NT], x0[MT], x1[MT]; unsigned sw, sx[MT]; } even, odd;
-    // step s is there, for every wave, and the fragments of step s - 1 have been read (so its buffer is free); the NBUF - 2 steps behind it may be on
-    // their way (fewer at the end: all of them are waited for)
-    auto arrive = [&](int s) {
-        if (s + NBUF - 2 < steps) wait_all_but<(NBUF - 2) * (T::PIECES + PS)>();
-        else wait_all_but<0>();
-        if (tail && s == steps - 1) {
+    // step s is there, for every wave, and the fragments of step s - 1 have been read (so its buffer is free)
+    auto arrive = [&](int s, auto ahead) {
+        if (s + decltype(ahead)::value < steps) landed(ahead);
+        else wait_all_but<0>();                                               // (fewer are under way at the end)
+        if (mine && s == steps - 1) {
 #pragma unroll
             for (int i = 0; i < T::PIECES; ++i)
-                if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(smem + buf * T::BUF + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
+                if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(ring + buf * T::BUF + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
     auto read = [&](Step& f) {
-        const char* const xa = smem + buf * T::BUF;
+        const char* const xa = ring + buf * T::BUF;
         const char* const wa = xa + BM * KROW;
         const unsigned* const scales = reinterpret_cast<const unsigned*>(xa + T::PANELS);
 #pragma unroll
@@ -419,28 +451,29 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
 #pragma unroll
         for (int i = 0; i < MT; ++i) { f.x0[i] = chunk(xa, wm + i * 16 + r, q); f.x1[i] = chunk(xa, wm + i * 16 + r, q + 4); }
         if (PS) {
-            f.sw = scales[T::SLOT / 4 - 64];
+            f.sw = scales[T::SA * 64];
 #pragma unroll
             for (int i = 0; i < MT; ++i) f.sx[i] = scales[wm + i * 16 + r];
         }
         buf = buf == NBUF - 1 ? 0 : buf + 1;
     };
     auto step = [&](int s, const Step& f, Step& next) {
-        if (s + 1 < steps) {
-            arrive(s + 1);
-            read(next);
+        if (s + 1 < rounds) {                                                 // (every group comes to every barrier)
+            arrive(s + 1, std::integral_constant<int, NBUF - 2>{});
+            if (s + 1 < steps) read(next);
         }
-        Frag<IN, EXACT> w[NT];
+        if (s >= steps) return;
         constexpr bool LATE = MT * NT < 16;                                   // (a second row of block sums would spill)
+        Frag<IN, EXACT> w[NT];
         f32x4 part[2][NT];
         Scale<IN, EXACT> sc[2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j].set(f.w0[j], f.w1[j]);
+        for (int j = 0; j < NT; ++j) w[j].set(f.w0[j], f.w1[j], f.sw);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             Frag<IN, EXACT> x;
-            x.set(f.x0[i], f.x1[i]);
-            if (PS) sc[i & 1].set(f.sw, f.sx[i]);
+            x.set(f.x0[i], f.x1[i], PS ? f.sx[i] : 0);
+            if (PS) sc[i & 1].set(f.sw, f.sx[i], bad[i]);
             mfma_row<IN, EXACT, NT>(acc[i], part[i & 1], w, x, sc[i & 1]);
             if (s + NBUF < steps) {                                           // requests between the instructions, some behind each row: the pipe is busy while they are issued
 #pragma unroll
@@ -449,7 +482,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
                     else asm volatile("" :: "v"(acc[i][j]));
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                bring(s + NBUF, i * ALL / MT, (i + 1) * ALL / MT);
+                bring(s + NBUF, i * T::PIECES / MT, (i + 1) * T::PIECES / MT);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (LATE && i > 0) fold_row<IN, EXACT, NT>(acc[i - 1], part[(i - 1) & 1], sc[(i - 1) & 1]);
@@ -457,26 +490,35 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
         }
         if (LATE) fold_row<IN, EXACT, NT>(acc[MT - 1], part[(MT - 1) & 1], sc[(MT - 1) & 1]);
     };
-    // (step 0 alone: NBUF steps are under way, and one fewer behind it than `arrive` counts on)
-    if (NBUF - 1 < steps) wait_all_but<(NBUF - 1) * (T::PIECES + PS)>();
-    else wait_all_but<0>();
-    if (tail && steps == 1) {
-#pragma unroll
-        for (int i = 0; i < T::PIECES; ++i)
-            if (tail_col(i) >= tail) *reinterpret_cast<i32x4*>(smem + (i * T::WAVES + wave) * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    read(even);
-    for (int s = 0; s < steps; s += 2) {
+    arrive(0, std::integral_constant<int, NBUF - 1>{});
+    if (steps > 0) read(even);
+    for (int s = 0; s < rounds; s += 2) {
         step(s, even, odd);
-        if (s + 1 < steps) step(s + 1, odd, even);
+        if (s + 1 < rounds) step(s + 1, odd, even);
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) spoil<IN, EXACT, NT>(acc[i], bad[i]);
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
+    if constexpr (KG == 2) {
+        f32x4* const sums = reinterpret_cast<f32x4*>(smem) + wave * MT * NT * 64 + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int i = 0; i < MT * NT; ++i) sums[i * 64] = acc[i / NT][i % NT];
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += sums[i * 64];
+        }
+        __syncthreads();
+        if (kg == 1) {
+            if (OUT == OUT_E4M3) __syncthreads();                             // (store_tile's)
+            return;
+        }
+    }
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
-// ---- the kernel for every case: 32 rows x 128 columns a workgroup, 32 columns a wave; operands through registers into LDS, from any alignment, two
-//      steps ahead in registers; two LDS buffers, one barrier a step
 struct AnyTile {
     static constexpr int WM = 1, WN = 4, MT = 2, NT = 2, BM = 32, BN = 128, WAVES = 4, LDS = 2 * (BM + BN) * KROW;
 };
@@ -529,6 +571,7 @@ __global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
     };
 
     f32x4 acc[2][2];
+    unsigned bad[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto step = [&](int s, Step& f) {
@@ -540,13 +583,13 @@ __global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
         __syncthreads();
         Frag<IN, EXACT> w[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { const int wr = BM + wave * 32 + j * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4)); }
+        for (int j = 0; j < 2; ++j) { const int wr = BM + wave * 32 + j * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4), sw); }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             Frag<IN, EXACT> x;
-            x.set(chunk(lds, i * 16 + r, q), chunk(lds, i * 16 + r, q + 4));
+            x.set(chunk(lds, i * 16 + r, q), chunk(lds, i * 16 + r, q + 4), sx[i]);
             Scale<IN, EXACT> sc;
-            if (IN != IN_BF16) sc.set(sw, sx[i]);
+            if (IN != IN_BF16) sc.set(sw, sx[i], bad[i]);
             mac_row<IN, EXACT, 2>(acc[i], w, x, sc);
         }
     };
@@ -557,6 +600,8 @@ __global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
         step(s, even);
         if (s + 1 < steps) step(s + 1, odd);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) spoil<IN, EXACT, 2>(acc[i], bad[i]);
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
@@ -654,10 +699,13 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
     };
 
     f32x4 acc[MT][NT];
+    unsigned bad[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
+        bad[i] = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     bring(0, 0, 0, ALL);
     if (steps > 1) { bring(1, 1, 0, ALL); wait_all_but<ALL>(); }
     else wait_all_but<0>();
@@ -679,17 +727,17 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
         for (int h = 0; h < H; ++h) {
             // ---- L
             if (h == 0) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4));
                 if (PS) sw = scales[BM + wn / BLK];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) w[j].set(chunk(wa, wn + j * 16 + r, q), chunk(wa, wn + j * 16 + r, q + 4), sw);
             }
             Frag<IN, EXACT> x[XG];
             unsigned sv[XG];
 #pragma unroll
             for (int i = 0; i < XG; ++i) {
                 const int row = wm + (h * XG + i) * 16 + r;
-                x[i].set(chunk(xa, row, q), chunk(xa, row, q + 4));
                 if (PS) sv[i] = scales[row];
+                x[i].set(chunk(xa, row, q), chunk(xa, row, q + 4), PS ? sv[i] : 0);
             }
             if (h == H - 1 && grp == 1) {                                     // step s + 1 is there but for what was asked for after it
                 if (!more) wait_all_but<0>();
@@ -703,7 +751,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             Scale<IN, EXACT> sc[2];
 #pragma unroll
             for (int i = 0; i < XG; ++i) {
-                if (PS) sc[i & 1].set(sw, sv[i]);
+                if (PS) sc[i & 1].set(sw, sv[i], bad[h * XG + i]);
                 mfma_row<IN, EXACT, NT>(acc[h * XG + i], part[i & 1], w, x[i], sc[i & 1]);
                 // requests between the instructions, a few behind each row: the pipe is busy while they are issued
                 int next = s + 2;
@@ -741,6 +789,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
         buf = buf == NBUF - 1 ? 0 : buf + 1;
     }
     if (grp == 0) phase_end();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) spoil<IN, EXACT, NT>(acc[i], bad[i]);
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
@@ -769,9 +819,13 @@ __global__ __launch_bounds__(1024) void product_rows_kernel(ProductArgs p)
         x_row[i] = p.a + src[i] * p.a_row;
     }
     const long long sb0 = g * p.sb_group + (long long)(n0 / BLK) * p.sb_row;
-    f32x4 acc[MT][1];
+    f32x4 bias;                                                               // (asked for here, used at the end)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i) bias[i] = p.bias && n0 + q * 4 + i < p.n ? p.bias[g * p.bias_group + n0 + q * 4 + i] : 0.f;
+    f32x4 acc[MT][1];
+    unsigned bad[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) { acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f}; bad[i] = 0; }
     for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
         i32x4 w[U][2], x[U][MT][2];
         unsigned sw[U], sx[U][MT];
@@ -804,32 +858,45 @@ __global__ __launch_bounds__(1024) void product_rows_kernel(ProductArgs p)
         for (int u = 0; u < U; ++u)
             if (s0 + u * WAVES < steps) {
                 Frag<IN, EXACT> wf[1], xf;
-                wf[0].set(w[u][0], w[u][1]);
+                wf[0].set(w[u][0], w[u][1], IN != IN_BF16 ? sw[u] : 0);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    xf.set(x[u][i][0], x[u][i][1]);
+                    xf.set(x[u][i][0], x[u][i][1], IN != IN_BF16 ? sx[u][i] : 0);
                     Scale<IN, EXACT> sc;
-                    if (IN != IN_BF16) sc.set(sw[u], sx[u][i]);
+                    if (IN != IN_BF16) sc.set(sw[u], sx[u][i], bad[i]);
                     mac_row<IN, EXACT, 1>(acc[i], wf, xf, sc);
                 }
             }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i][0];
+    for (int i = 0; i < MT; ++i) { spoil<IN, EXACT, 1>(acc[i], bad[i]); part[wave][i][lane] = acc[i][0]; }
     __syncthreads();
     if (threadIdx.x >= MT * 64) return;
-    const int j = first + wave * 16 + r;                                      // (waves 0 .. MT - 1: a row tile each)
+    const int j = first + wave * 16 + r, col = n0 + q * 4;                    // (waves 0 .. MT - 1: a row tile each)
     f32x4 y = part[0][wave][lane];
 #pragma unroll
     for (int u = 1; u < WAVES; ++u) y += part[u][wave][lane];
     if (j >= end) return;
     if (p.index && source_row(p, j, end) < 0) y = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int col = n0 + q * 4;
-    y = finish(p, y, p.bias ? p.bias + g * p.bias_group : nullptr, col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { y[i] += bias[i]; if (p.relu) y[i] = y[i] < 0.f ? 0.f : y[i]; }          // (NaN stays)
     if (col < p.n) store4<OUT>(p, j, col, y, wide_stores(p, OUT == OUT_F32 ? 16 : 8));
 }
 
 namespace {
+
+// a kernel's LDS beyond the default, once for each device
+hipError_t allow_lds(const void* kernel, int bytes, std::atomic<unsigned long long>& devices)
+{
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (devices.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 long long row_tiles(const ProductArgs& p, int bm)                             // at most: a group of rows ends inside a tile
 {
@@ -852,8 +919,9 @@ hipError_t launch_ring(ProductArgs p, hipStream_t st)
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(product_ring_kernel<IN, OUT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-    if (once != hipSuccess) return once;
+    static std::atomic<unsigned long long> devices{0};
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(product_ring_kernel<IN, OUT, T>), T::LDS, devices);
+    if (e != hipSuccess) return e;
     product_ring_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
@@ -864,8 +932,9 @@ hipError_t launch_phased(ProductArgs p, hipStream_t st)
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(product_phased_kernel<IN, OUT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
-    if (once != hipSuccess) return once;
+    static std::atomic<unsigned long long> devices{0};
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(product_phased_kernel<IN, OUT, T>), T::LDS, devices);
+    if (e != hipSuccess) return e;
     product_phased_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
@@ -883,20 +952,24 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 // Which kernel: the one with the least estimated time, 2 us + rounds of 256 tiles x (a tile's beginning and end + its steps).  The microseconds below are
 // fitted to runs on 1 .. 32768 rows of 2048 x 4736 and 512 x 2048 and to grouped ones (a graph of 20 calls each; us):
 //
-//   rows            e4m3 to bf16: few rows   32 x 128   64 x 128   128 x 128   128 x 256   192 x 256   256 x 256
-//        1                             5.7       15.5       19.4        26.3        30.1                    50.7
-//       32                             7.4       15.7       19.4        26.3        30.4                    50.7
-//      128                            19.2       16.6                               30.7
-//     1024                                       33.8       22.4        28.8        33.4                    52.6
-//     2048                                       62.3       41.7        30.5        34.7        48.2        54.1
-//     4096                                      119.5       78.4        56.9        43.3        53.7        56.1
-//     5000                                                                          69.8        52.7        58.4
-//    32768                                       1015        652         452         303         301         254
+//   rows   e4m3 to bf16:   16 / 32 at a time   32 x 128   64 x 128   128 x 128   128 x 256   192 x 256   256 x 256
+//        1                       5.5 /  6.2       14.3       16.6        27.2
+//       32                       7.3 /  9.5       14.6       16.9        27.4
+//      128                      25.8 / 18.5       15.6       17.3        27.8        31.5        41.1        50.5
+//     1024                                        32.3       20.9        29.9        33.5        44.8        52.7
+//     2048                                        59.9       38.5        32.4        35.3        46.5        53.9
+//     4096                                       114.8       76.9        60.6        46.3        50.7        56.7
+//     5000                                       141.0       90.9        84.2        69.5        53.2        57.5
+//     8192                                                                           81.3        92.5        66.9
+//    32768                                       941.9      626.2       458.8       309.6       301.7       263.2
+//
+// Folded block sums (fp32 scales) take 1.05 .. 1.2 times as long, 16-bit operands from e4m3 (fp32 results) 1.4 times in the rings and 1.75 in the large
+// tiles (5.5 us at one row, 490 and 529 us at 32768), bf16 operands over the same K twice, since a step of K is 64 of theirs.
 template <int IN, int OUT>
 hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
     constexpr bool EXACT = OUT == OUT_F32;
-    constexpr int F = !FOLDS<IN, EXACT> ? 0 : !EXACT ? 1 : 2;                 // scales for the matrix instruction (or none) | block sums folded | e4m3 as fp16
+    constexpr int F = IN != IN_BF16 && EXACT ? 2 : FOLDS<IN, EXACT> ? 1 : 0;                 // scales for the matrix instruction (or none) | block sums folded | e4m3 as fp16
     if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
     const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // the ring's and the phased kernel's 32-bit offsets
@@ -914,25 +987,25 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     offer(ROWS16, OUT != OUT_E4M3, 16, 16, 1.5, aligned ? 0.13 : 0.2);
     offer(ROWS32, OUT != OUT_E4M3, 32, 16, 1.5, aligned ? 0.17 : 0.25);
     offer(ANY, !dma, 32, 128, 2, 1.3);
-    offer(R32, dma, 32, 128, 2, F == 0 ? 0.40 : F == 1 ? 0.46 : 0.63);
-    offer(R64, dma, 64, 128, 2, F == 0 ? 0.50 : F == 1 ? 0.58 : 0.92);
-    offer(R128, dma && F == 0, 128, 128, 3, 0.72);                            // (folding does not fit its registers)
-    offer(P128, whole, 128, 256, 4, F == 0 ? 1.06 : F == 1 ? 1.28 : 1.85);
-    offer(P192, whole && F < 2, 192, 256, 4, F == 0 ? 1.35 : 1.45);
-    offer(P256, whole && F < 2, 256, 256, 5, F == 0 ? 1.65 : 2.05);
+    offer(R32, dma, 32, 128, 2, F == 0 ? 0.35 : F == 1 ? 0.37 : 0.50);
+    offer(R64, dma, 64, 128, 2, F == 0 ? 0.44 : F == 1 ? 0.46 : 0.70);
+    offer(R128, dma && F == 0, 128, 128, 3, 0.69);                            // (folding does not fit its registers)
+    offer(P128, whole, 128, 256, 4, F == 0 ? 1.02 : F == 1 ? 1.15 : 1.92);
+    offer(P192, whole && F < 2, 192, 256, 4, F == 0 ? 1.28 : 1.45);
+    offer(P256, whole && F < 2, 256, 256, 5, F == 0 ? 1.57 : 1.95);
     if constexpr (OUT != OUT_E4M3) {
         if (best == ROWS16) return launch_rows<IN, OUT, 1, 3>(p, st);
         if (best == ROWS32) return launch_rows<IN, OUT, 2, 2>(p, st);
     }
     if constexpr (F == 0)
-        if (best == R128) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4>>(p, st);
+        if (best == R128) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4, 1>>(p, st);
     if constexpr (F < 2) {
         if (best == P192) return launch_phased<IN, OUT, Phased<2, 4, 6, 4, 2>>(p, st);
         if (best == P256) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
     }
     switch (best) {
-    case R32: return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 6>>(p, st);
-    case R64: return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 5>>(p, st);
+    case R32: return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 3, 2>>(p, st);
+    case R64: return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 3, 2>>(p, st);
     case P128: return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
     default: return launch_any<IN, OUT>(p, st);
     }
