@@ -255,7 +255,8 @@ template <int WM_, int WN_, int MT_, int NT_, int NBUF_, int KG_> struct Ring {
 };
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
-// sixteen rows at a time round in its own corner of LDS (a lane holds four columns of a row, a store takes neighbouring lanes along a row).
+// sixteen rows at a time round in its own corner of LDS (a lane holds four columns of a row, a store takes neighbouring lanes along a row).  Rows of y that
+// do not start at multiples of four values are stored value by value.
 template <int IN, int OUT, class T>
 __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T::MT][T::NT], char* smem, int g, int first, int end, int n0, int wave, int lane)
 {
@@ -317,7 +318,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
 #pragma unroll
     for (int i = 0; i < T::MT; ++i) {
         const int j0 = first + wm + i * 16;
-        if (whole) {
+        if (whole || !wide) {
 #pragma unroll
             for (int u = 0; u < T::NT; ++u) {
                 char* at = turn + r * PITCH + (u * 16 + q * 4) * SZ;
@@ -327,13 +328,23 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
                 else *reinterpret_cast<int*>(at) = to_e4m3x4(acc[i][u][0], acc[i][u][1], acc[i][u][2], acc[i][u][3]);
             }
             __builtin_amdgcn_wave_barrier();
-            constexpr int CH = ROW / 16;                                      // 16-byte pieces of a row
+            if (whole) {
+                constexpr int CH = ROW / 16;                                  // 16-byte pieces of a row
 #pragma unroll
-            for (int t = 0; t < (CH * 16 + 63) / 64; ++t) {
-                const int row = (t * 64 + lane) / CH, c = (t * 64 + lane) % CH;
-                if (row >= 16) break;
-                const i32x4 v = *reinterpret_cast<const i32x4*>(turn + row * PITCH + c * 16);
-                if (j0 + row < end) *reinterpret_cast<i32x4*>(y0 + (long long)(j0 + row) * p.y_row + c * 16) = v;
+                for (int t = 0; t < (CH * 16 + 63) / 64; ++t) {
+                    const int row = (t * 64 + lane) / CH, c = (t * 64 + lane) % CH;
+                    if (row >= 16) break;
+                    const i32x4 v = *reinterpret_cast<const i32x4*>(turn + row * PITCH + c * 16);
+                    if (j0 + row < end) *reinterpret_cast<i32x4*>(y0 + (long long)(j0 + row) * p.y_row + c * 16) = v;
+                }
+            } else {                                                          // (neighbouring lanes: neighbouring values of a row)
+                using E = std::conditional_t<OUT == OUT_F32, float, std::conditional_t<OUT == OUT_BF16, unsigned short, char>>;
+#pragma unroll 4
+                for (int t = 0; t < T::NT * 4; ++t) {
+                    const int row = (t * 64 + lane) / (T::NT * 16), c = (t * 64 + lane) % (T::NT * 16);
+                    const E v = *reinterpret_cast<const E*>(turn + row * PITCH + c * SZ);
+                    if (j0 + row < end && n0 + wn + c < p.n) *reinterpret_cast<E*>(y0 + (long long)(j0 + row) * p.y_row + c * SZ) = v;
+                }
             }
             __builtin_amdgcn_wave_barrier();
         } else if (j0 + r < end) {
@@ -519,81 +530,110 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
-struct AnyTile {
-    static constexpr int WM = 1, WN = 4, MT = 2, NT = 2, BM = 32, BN = 128, WAVES = 4, LDS = 2 * (BM + BN) * KROW;
+// ---- the kernel for operands at any address: panels come through registers as whole words, two steps ahead, and are shifted to their bytes on the way to
+//      LDS (16-byte loads that do not start at a word take longer: 733 rows of 1001 x 1419 to fp32 22.6 us with them and a last step byte by byte, 14.5
+//      so).  A lane's last word is its neighbour's first.
+template <int WM_, int WN_, int MT_, int NT_> struct Any {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int AT_ONCE = THREADS / 8, CH = (BM + BN) / AT_ONCE, LDS = 2 * (BM + BN) * KROW;   // rows that all threads bring together; 16-byte chunks a thread and step
+    static_assert(BN == BLK && BM % AT_ONCE == 0 && BN % AT_ONCE == 0, "tile");
 };
 
-template <int IN, int OUT>
-__global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
+template <int IN, int OUT, class T>
+__global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs p)
 {
-    constexpr int BM = 32, BN = 128, CH = (BM + BN) * 8 / 256;               // 16-byte chunks a thread brings each step
+    constexpr int BM = T::BM, BN = T::BN, CH = T::CH, MT = T::MT, NT = T::NT;
     constexpr bool EXACT = OUT == OUT_F32;
-    using T = AnyTile;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     Place at;
     if (!find_tile(p, BM, at)) return;
     const int g = at.g, first = at.first, end = at.end, tn = at.tn;
     const int n0 = tn * BN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    const int steps = (p.kbytes + KROW - 1) / KROW;
+    const int wm = (wave / T::WN) * MT * 16, wn = (wave % T::WN) * NT * 16;
+    const int steps = p.a_rows ? (p.kbytes + KROW - 1) / KROW : 0;
 
-    const char* row[CH];                                                      // null: a row of zeros
+    const char* row[CH];                                                      // (rows without a source and columns behind the last: any, not stored or taken out at the end)
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-        const int lr = (int)(threadIdx.x >> 3) + 32 * i;
-        row[i] = nullptr;
-        if (lr < BM) { const long long s = source_row(p, first + lr, end); if (s >= 0) row[i] = p.a + s * p.a_row; }
-        else if (n0 + lr - BM < p.n) row[i] = p.b + g * p.b_group + (long long)(n0 + lr - BM) * p.b_row;
+        const int lr = (int)(threadIdx.x >> 3) + T::AT_ONCE * i;
+        if (lr < BM) { const long long s = source_row(p, first + lr, end); row[i] = p.a + (s < 0 ? 0 : s) * p.a_row; }
+        else { const int c = n0 + lr - BM; row[i] = p.b + g * p.b_group + (long long)(c < p.n ? c : p.n - 1) * p.b_row; }
     }
     const int c8 = threadIdx.x & 7;
-    long long mine[2];                                                        // the rows whose scales this lane applies
+    long long mine[MT];                                                       // the rows whose scales this lane applies
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mine[i] = source_row(p, first + i * 16 + r, end);
+    for (int i = 0; i < MT; ++i) { const long long s = source_row(p, first + wm + i * 16 + r, end); mine[i] = s < 0 ? 0 : s; }
     const long long sb0 = g * p.sb_group + (long long)tn * p.sb_row;
-    struct Step { i32x4 v[CH]; unsigned sw, sx[2]; } even, odd;
+    struct Step { i32x4 v[CH]; int next[CH]; unsigned sw, sx[MT]; } even, odd;
     auto fetch = [&](int s, Step& f) {
+        const int from = s * KROW + c8 * 16;
         if ((s + 1) * KROW <= p.kbytes) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) f.v[i] = row[i] ? load16(row[i] + s * KROW + c8 * 16) : i32x4{0, 0, 0, 0};
+            for (int i = 0; i < CH; ++i) __builtin_memcpy(&f.v[i], __builtin_assume_aligned(word_of(row[i]) + from, 4), 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) f.v[i] = row[i] ? load16_tail(row[i], s * KROW + c8 * 16, p.kbytes) : i32x4{0, 0, 0, 0};
+            for (int i = 0; i < CH; ++i) {
+                const int last = last_word(row[i], p.kbytes);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f.v[i][j] = word_at(word_of(row[i]), from + 4 * j < last ? from + 4 * j : last);
+            }
+        }
+        if (c8 == 7) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) { const int last = last_word(row[i], p.kbytes); f.next[i] = word_at(word_of(row[i]), from + 16 < last ? from + 16 : last); }
         }
         if constexpr (IN == IN_F8_F32) {
             f.sw = static_cast<const unsigned*>(p.sb)[sb0 + s];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) f.sx[i] = mine[i] >= 0 ? static_cast<const unsigned*>(p.sa)[s * p.sa_block + mine[i]] : 0x3f800000u;
+            for (int i = 0; i < MT; ++i) f.sx[i] = static_cast<const unsigned*>(p.sa)[s * p.sa_block + mine[i]];
         }
         if constexpr (IN == IN_F8_E8) {
             f.sw = static_cast<const unsigned char*>(p.sb)[sb0 + s];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) f.sx[i] = mine[i] >= 0 ? static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine[i]] : 127u;
+            for (int i = 0; i < MT; ++i) f.sx[i] = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + mine[i]];
         }
     };
 
-    f32x4 acc[2][2];
-    unsigned bad[2] = {0, 0};
+    f32x4 acc[MT][NT];
+    unsigned bad[MT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MT; ++i) {
+        bad[i] = 0;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     auto step = [&](int s, Step& f) {
         char* const lds = smem + (s & 1) * (BM + BN) * KROW;                  // (last read two steps ago: a barrier lies between)
+        const int left = p.kbytes - s * KROW - c8 * 16;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) *reinterpret_cast<i32x4*>(lds + slot_of((int)(threadIdx.x >> 3) + 32 * i, c8)) = f.v[i];
-        const unsigned sw = f.sw, sx[2] = {f.sx[0], f.sx[1]};
+        for (int i = 0; i < CH; ++i) {
+            const int over = __builtin_amdgcn_update_dpp(0, f.v[i][0], 0x101, 0xf, 0xf, false);          // the next lane's first word
+            i32x4 v = shift_words(f.v[i], c8 == 7 ? f.next[i] : over, (unsigned)reinterpret_cast<uintptr_t>(row[i]) & 3);
+            if ((s + 1) * KROW > p.kbytes) v = cut_bytes(v, left);
+            *reinterpret_cast<i32x4*>(lds + slot_of((int)(threadIdx.x >> 3) + T::AT_ONCE * i, c8)) = v;
+        }
+        unsigned sw = f.sw, sx[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sx[i] = f.sx[i];
         if (s + 2 < steps) fetch(s + 2, f);
         __syncthreads();
-        Frag<IN, EXACT> w[2];
+        Frag<IN, EXACT> w[NT];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { const int wr = BM + wave * 32 + j * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4), sw); }
+        for (int j = 0; j < NT; ++j) { const int wr = BM + wn + j * 16 + r; w[j].set(chunk(lds, wr, q), chunk(lds, wr, q + 4), sw); }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < MT; ++i) {
             Frag<IN, EXACT> x;
-            x.set(chunk(lds, i * 16 + r, q), chunk(lds, i * 16 + r, q + 4), sx[i]);
+            x.set(chunk(lds, wm + i * 16 + r, q), chunk(lds, wm + i * 16 + r, q + 4), sx[i]);
             Scale<IN, EXACT> sc;
             if (IN != IN_BF16) sc.set(sw, sx[i], bad[i]);
-            mac_row<IN, EXACT, 2>(acc[i], w, x, sc);
+            mac_row<IN, EXACT, NT>(acc[i], w, x, sc);
         }
     };
-    even.sw = odd.sw = even.sx[0] = even.sx[1] = odd.sx[0] = odd.sx[1] = 0;
+    even.sw = odd.sw = 0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) even.sx[i] = odd.sx[i] = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) even.next[i] = odd.next[i] = 0;
     if (steps > 0) fetch(0, even);
     if (steps > 1) fetch(1, odd);
     for (int s = 0; s < steps; s += 2) {
@@ -601,7 +641,7 @@ __global__ __launch_bounds__(256, 2) void product_any_kernel(ProductArgs p)
         if (s + 1 < steps) step(s + 1, odd);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) spoil<IN, EXACT, 2>(acc[i], bad[i]);
+    for (int i = 0; i < MT; ++i) spoil<IN, EXACT, NT>(acc[i], bad[i]);
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
@@ -903,13 +943,14 @@ long long row_tiles(const ProductArgs& p, int bm)                             //
     return p.offsets ? (long long)p.m / bm + (p.groups < p.m ? p.groups : p.m) : ((long long)p.m + bm - 1) / bm;
 }
 
-template <int IN, int OUT>
+template <int IN, int OUT, class T>
 hipError_t launch_any(ProductArgs p, hipStream_t st)
 {
-    p.tiles_n = (p.n + AnyTile::BN - 1) / AnyTile::BN;
-    const long long grid = (row_tiles(p, AnyTile::BM) * p.tiles_n + 7) / 8 * 8;
+    p.tiles_n = (p.n + T::BN - 1) / T::BN;
+    const long long grid = (row_tiles(p, T::BM) * p.tiles_n + 7) / 8 * 8;
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    product_any_kernel<IN, OUT><<<(unsigned)grid, 256, AnyTile::LDS, st>>>(p);
+    static_assert(T::LDS <= 64 * 1024, "LDS");
+    product_any_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
 
@@ -963,6 +1004,9 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 //     8192                                                                           81.3        92.5        66.9
 //    32768                                       941.9      626.2       458.8       309.6       301.7       263.2
 //
+// Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 12.1 | 17.2, 1500 16.1 | 17.6, 3000 23.7 | 19.5, 20000 118 | 93;
+// 4096 166.9 | 99.5.
+//
 // Folded block sums (fp32 scales) take 1.05 .. 1.2 times as long, 16-bit operands from e4m3 (fp32 results) 1.4 times in the rings and 1.75 in the large
 // tiles (5.5 us at one row, 490 and 529 us at 32768), bf16 operands over the same K twice, since a step of K is 64 of theirs.
 template <int IN, int OUT>
@@ -970,12 +1014,12 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
     constexpr bool EXACT = OUT == OUT_F32;
     constexpr int F = IN != IN_BF16 && EXACT ? 2 : FOLDS<IN, EXACT> ? 1 : 0;                 // scales for the matrix instruction (or none) | block sums folded | e4m3 as fp16
-    if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT>(p, st);
+    if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT, Any<1, 4, 2, 2>>(p, st);
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
     const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // the ring's and the phased kernel's 32-bit offsets
     const bool dma = aligned && near, whole = dma && p.kbytes % KROW == 0;
     const double steps = (p.kbytes + KROW - 1) / KROW;
-    enum { ROWS16, ROWS32, ANY, R32, R64, R128, P128, P192, P256 };
+    enum { ROWS16, ROWS32, ANY, ANY128, R32, R64, R128, P128, P192, P256 };
     int best = -1;
     double least = 0;
     auto offer = [&](int kernel, bool can, int bm, int bn, double edge, double step) {
@@ -986,7 +1030,8 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     };
     offer(ROWS16, OUT != OUT_E4M3, 16, 16, 1.5, aligned ? 0.13 : 0.2);
     offer(ROWS32, OUT != OUT_E4M3, 32, 16, 1.5, aligned ? 0.17 : 0.25);
-    offer(ANY, !dma, 32, 128, 2, 1.3);
+    offer(ANY, !dma, 32, 128, 2, F ? 0.6 : 0.5);                              // (several at once on a CU)
+    offer(ANY128, !dma, 128, 128, 3, F ? 1.65 : 1.2);
     offer(R32, dma, 32, 128, 2, F == 0 ? 0.35 : F == 1 ? 0.37 : 0.50);
     offer(R64, dma, 64, 128, 2, F == 0 ? 0.44 : F == 1 ? 0.46 : 0.70);
     offer(R128, dma && F == 0, 128, 128, 3, 0.69);                            // (folding does not fit its registers)
@@ -1007,7 +1052,8 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     case R32: return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 3, 2>>(p, st);
     case R64: return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 3, 2>>(p, st);
     case P128: return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
-    default: return launch_any<IN, OUT>(p, st);
+    case ANY128: return launch_any<IN, OUT, Any<2, 4, 4, 2>>(p, st);
+    default: return launch_any<IN, OUT, Any<1, 4, 2, 2>>(p, st);
     }
 }
 

@@ -52,14 +52,34 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // 16 bytes from any address (global memory serves unaligned 16-byte loads)
 __device__ __forceinline__ i32x4 load16(const char* p) { i32x4 v; __builtin_memcpy(&v, p, 16); return v; }
-// bytes [at, at + 16) of a row that ends at byte `end`: what lies behind it reads as zero
+// Bytes of a row at any address from whole words: those that hold them, and no word that holds none of the row's.  `row` & 3 is the shift.
+__device__ __forceinline__ const char* word_of(const char* row) { return row - (reinterpret_cast<uintptr_t>(row) & 3); }
+__device__ __forceinline__ int last_word(const char* row, int end) { return (end - 1 + (int)(reinterpret_cast<uintptr_t>(row) & 3)) & ~3; }
+__device__ __forceinline__ int word_at(const char* words, int at) { return *reinterpret_cast<const int*>(words + at); }
+// words w[0 .. 4] -> sixteen bytes; what lies at `left` or behind it reads as zero
+__device__ __forceinline__ i32x4 shift_words(i32x4 w, int next, unsigned by)
+{
+    return i32x4{(int)__builtin_amdgcn_alignbyte(w[1], w[0], by), (int)__builtin_amdgcn_alignbyte(w[2], w[1], by), (int)__builtin_amdgcn_alignbyte(w[3], w[2], by),
+                 (int)__builtin_amdgcn_alignbyte(next, w[3], by)};
+}
+__device__ __forceinline__ i32x4 cut_bytes(i32x4 v, int left)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = left - 4 * i;
+        v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & ((1 << 8 * n) - 1);
+    }
+    return v;
+}
+// bytes [at, at + 16) of a row that ends at byte `end` > 0: what lies behind it reads as zero
 __device__ __forceinline__ i32x4 load16_tail(const char* row, int at, int end)
 {
-    i32x4 v = {0, 0, 0, 0};
-    unsigned char* b = reinterpret_cast<unsigned char*>(&v);
-    if (at + 16 <= end) return load16(row + at);
-    for (int i = 0; i < 16; ++i) if (at + i < end) b[i] = (unsigned char)row[at + i];
-    return v;
+    const char* const words = word_of(row);
+    const int last = last_word(row, end);
+    i32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = word_at(words, at + 4 * i < last ? at + 4 * i : last);
+    return cut_bytes(shift_words(w, word_at(words, at + 16 < last ? at + 16 : last), (unsigned)reinterpret_cast<uintptr_t>(row) & 3), end - at);
 }
 
 // The scale of a block whose largest finite magnitude is `most`: the smallest e with most <= 448 * 2^e.  most = f * 2^p with f in [0.5, 1) and
