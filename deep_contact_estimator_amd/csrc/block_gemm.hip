@@ -646,7 +646,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
-// ---- the kernel for chip-filling products (K a multiple of 128 bytes, operands within 4 GB): eight waves in two groups that are a phase apart.
+// ---- the kernel for chip-filling products (operands within 4 GB): eight waves in two groups that are a phase apart.
 //
 // Waves w and w + 4 share a SIMD.  While one group's phase is its matrix instructions, the other group's is reads of fragments from LDS and waits: the
 // matrix pipe passes from one group to the other without a pause, and no wave waits for LDS with the pipe idle.  A step of group 0 is L0 M0 .. (of
@@ -656,14 +656,16 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
 // 64 KB a step and CU are 1 us of what L2 gives to all CUs at once (measured, 17 TB/s) and another half before the first of them is there, against 0.9 us
 // of matrix instructions: panels have to be asked for more than a step ahead.  256 x 256 tiles leave room for two buffers, so each part of a panel is
 // asked for once its buffer has been read for the last time, a quarter of a step's requests (they take the CU 1150 cycles in all) in every phase: of step
-// s + 2, group 1's half of the weights at phase 4s + 2, group 0's rows at 4s + 3, group 1's at 4s + 4, group 0's half of the weights at 4s + 5.  128 x 256 tiles have three buffers: step s + 2 at phase 2H s + 1, by group 1 at 2H s.  All of it between matrix
-// instructions.  Scales come the same way, a word a row.
+// s + 2, group 1's half of the weights at phase 4s + 2, group 0's rows at 4s + 3, group 1's at 4s + 4, group 0's half of the weights at 4s + 5.  Smaller
+// tiles have three buffers: step s + 2 at phase 2H s + 1, by group 1 at 2H s.  All of it between matrix instructions.  Scales come the same way, a word
+// a row.
 template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
     static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BUF = (BM + BN) * KROW, PA = BM / 64, PB = BN / 64;   // pieces of eight rows a wave brings: of its group's rows, of the weights
     static constexpr int SLOT = (BM + 64) * 4;                                // a step's scales: the rows', the column blocks'
     static constexpr int LDS = NBUF * BUF + 4 * SLOT;
+    template <int IN> static constexpr bool TAIL = !(MT == 8 && IN == IN_F8_F32);   // (no register left where block sums are folded)
     static_assert(WM == 2 && WN == 4 && BN / BLK <= 64 && (NBUF == 2 || NBUF == 3), "two groups of four waves");
 };
 
@@ -680,12 +682,14 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
     const int g = place.g, first = place.first, end = place.end, n0 = place.tn * T::BN;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, q = lane >> 4;
     const int grp = wave >> 2, w4 = wave & 3, wm = grp * MT * 16, wn = w4 * NT * 16;
-    const int steps = p.kbytes / KROW;
+    const int steps = (p.kbytes + KROW - 1) / KROW, tail = T::template TAIL<IN> ? p.kbytes % KROW : 0;      // (tail: bytes of the last step, where K ends inside it)
 
+    const int col = ((lane & 7) ^ ((w4 & 1) * 4 + (lane >> 4))) * 16;         // this lane's chunk of a row (a wave's pieces of eight rows are all even ones or all odd ones)
+    const bool cut = tail && col >= tail;                                     // ... lies behind the end in the last step: the first is read in its place and made zeros
     unsigned from[PA + PB];                                                   // from the step's column of a, of the group's b
 #pragma unroll
     for (int i = 0; i < PA + PB; ++i) {
-        const int lr = (i < PA ? grp * (BM / 16) + i * 4 + w4 : (i - PA) * 8 + wave) * 8 + (lane >> 3), col = ((lane & 7) ^ ((lr >> 1) & 7)) * 16;
+        const int lr = (i < PA ? grp * (BM / 16) + i * 4 + w4 : (i - PA) * 8 + wave) * 8 + (lane >> 3);
         unsigned row;
         if (i < PA) { const long long s = source_row(p, first + lr, end); row = (unsigned)(s < 0 ? 0 : s) * (unsigned)p.a_row; }
         else { const int c = n0 + lr; row = (unsigned)(c < p.n ? c : p.n - 1) * (unsigned)p.b_row; }
@@ -718,12 +722,21 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
 #pragma unroll
         for (int t = 0; t < PB + PS + PA; ++t) {
             if (t < lo || t >= hi) continue;
+            if (tail && s == steps - 1 && (t < PB || t >= PB + PS)) from[t < PB ? PA + t : t - PB - PS] -= cut ? col : 0;
             if (t < PB) dma16s(b0 + (long long)s * KROW, from[PA + t], lds0 + buf * T::BUF + (BM / 8 + t * 8 + wave) * 1024);
             else if (t < PB + PS) {
                 const unsigned to = lds0 + NBUF * T::BUF + (s & 3) * T::SLOT + s_to;
                 if constexpr (SZ == 4) dma4s(s_from + s * s_step, s_at, to);
                 else dma1s(s_from + s * s_step, s_at, to);
             } else dma16s(p.a + (long long)s * KROW, from[t - PB - PS], lds0 + buf * T::BUF + (grp * (BM / 16) + (t - PB - PS) * 4 + w4) * 1024);
+        }
+    };
+    auto clear_tail = [&](int buf) {                                          // once this wave's pieces of the last step are there, before the barrier that says so
+        if (!cut) return;
+#pragma unroll
+        for (int t = 0; t < PA + PB; ++t) {
+            const int piece = t < PA ? grp * (BM / 16) + t * 4 + w4 : BM / 8 + (t - PA) * 8 + wave;
+            *reinterpret_cast<i32x4*>(smem + buf * T::BUF + piece * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
         }
     };
     constexpr int ALL = PB + PS + PA;
@@ -748,7 +761,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
     }
     bring(0, 0, 0, ALL);
     if (steps > 1) { bring(1, 1, 0, ALL); wait_all_but<ALL>(); }
-    else wait_all_but<0>();
+    else { wait_all_but<0>(); clear_tail(0); }
     phase_end();
     if (grp == 1) {
         if (NBUF == 3 && steps > 2) bring(2, 2, 0, ALL);
@@ -761,6 +774,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
         const char* const wa = xa + BM * KROW;
         const unsigned* const scales = reinterpret_cast<const unsigned*>(smem + NBUF * T::BUF + (s & 3) * T::SLOT);
         const bool more = s + 2 < steps;
+        const int buf1 = buf == NBUF - 1 ? 0 : buf + 1;
         Frag<IN, EXACT> w[NT];
         unsigned sw = 0;
 #pragma unroll
@@ -783,6 +797,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
                 if (!more) wait_all_but<0>();
                 else if (NBUF == 3) wait_all_but<ALL>();
                 else wait_all_but<PB>();
+                if (s + 2 == steps) clear_tail(buf1);
             }
             phase_end();
             // ---- M
@@ -823,10 +838,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
                 if (!more) wait_all_but<0>();
                 else if (NBUF == 3) wait_all_but<ALL>();
                 else wait_all_but<PA + PS>();
+                if (s + 2 == steps) clear_tail(buf1);
             }
             phase_end();
         }
-        buf = buf == NBUF - 1 ? 0 : buf + 1;
+        buf = buf1;
     }
     if (grp == 0) phase_end();
 #pragma unroll
@@ -994,21 +1010,23 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 // fitted to runs on 1 .. 32768 rows of 2048 x 4736 and 512 x 2048 and to grouped ones (a graph of 20 calls each; us):
 //
 //   rows   e4m3 to bf16:   16 / 32 at a time   32 x 128   64 x 128   128 x 128   128 x 256   192 x 256   256 x 256
-//        1                       5.5 /  6.2       14.3       16.6        27.2
-//       32                       7.3 /  9.5       14.6       16.9        27.4
-//      128                      25.8 / 18.5       15.6       17.3        27.8        31.5        41.1        50.5
-//     1024                                        32.3       20.9        29.9        33.5        44.8        52.7
-//     2048                                        59.9       38.5        32.4        35.3        46.5        53.9
-//     4096                                       114.8       76.9        60.6        46.3        50.7        56.7
-//     5000                                       141.0       90.9        84.2        69.5        53.2        57.5
+//        1                       5.5 /  6.2       14.3       16.6
+//       32                       7.3 /  9.5       14.6       16.9
+//      128                      25.8 / 18.5       15.6       17.3                    31.5        41.1        50.5
+//     1024                                        32.3       20.9        24.6        33.5        44.8        52.7
+//     1571                                                   31.3        28.0
+//     2048                                        59.9       38.5        30.1        35.3        46.5        53.9
+//     4096                                       114.8       76.9        53.9        46.3        50.7        56.7
+//     5000                                       141.0       90.9                    69.5        53.2        57.5
 //     8192                                                                           81.3        92.5        66.9
-//    32768                                       941.9      626.2       458.8       309.6       301.7       263.2
+//    32768                                       941.9      626.2       409         309.6       301.7       263.2
 //
 // Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 12.1 | 17.2, 1500 16.1 | 17.6, 3000 23.7 | 19.5, 20000 118 | 93;
 // 4096 166.9 | 99.5.
 //
-// Folded block sums (fp32 scales) take 1.05 .. 1.2 times as long, 16-bit operands from e4m3 (fp32 results) 1.4 times in the rings and 1.75 in the large
-// tiles (5.5 us at one row, 490 and 529 us at 32768), bf16 operands over the same K twice, since a step of K is 64 of theirs.
+// Folded block sums (fp32 scales) take 1.05 .. 1.2 times as long, 16-bit operands from e4m3 (fp32 results) 1.4 times in the rings and 1.6 .. 1.9 in the
+// large tiles (1571 rows 41 us, 32768 490 with e8m0 scales and 529 with fp32 ones), bf16 operands over the same K twice, since a step of K is 64 of theirs.
+// A K that ends inside a step costs up to 5 % (4720 instead of 4736: 4096 rows 47.4 us, not 42.5 .. 46).
 template <int IN, int OUT>
 hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
@@ -1017,9 +1035,9 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT, Any<1, 4, 2, 2>>(p, st);
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
     const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // the ring's and the phased kernel's 32-bit offsets
-    const bool dma = aligned && near, whole = dma && p.kbytes % KROW == 0;
+    const bool dma = aligned && near;
     const double steps = (p.kbytes + KROW - 1) / KROW;
-    enum { ROWS16, ROWS32, ANY, ANY128, R32, R64, R128, P128, P192, P256 };
+    enum { ROWS16, ROWS32, ANY, ANY128, R32, R64, P128N, P128, P192, P256 };
     int best = -1;
     double least = 0;
     auto offer = [&](int kernel, bool can, int bm, int bn, double edge, double step) {
@@ -1034,16 +1052,14 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     offer(ANY128, !dma, 128, 128, 3, F ? 1.65 : 1.2);
     offer(R32, dma, 32, 128, 2, F == 0 ? 0.35 : F == 1 ? 0.37 : 0.50);
     offer(R64, dma, 64, 128, 2, F == 0 ? 0.44 : F == 1 ? 0.46 : 0.70);
-    offer(R128, dma && F == 0, 128, 128, 3, 0.69);                            // (folding does not fit its registers)
-    offer(P128, whole, 128, 256, 4, F == 0 ? 1.02 : F == 1 ? 1.15 : 1.92);
-    offer(P192, whole && F < 2, 192, 256, 4, F == 0 ? 1.28 : 1.45);
-    offer(P256, whole && F < 2, 256, 256, 5, F == 0 ? 1.57 : 1.95);
+    offer(P128N, dma, 128, 128, 3, F == 0 ? 0.68 : F == 1 ? 0.70 : 1.22);
+    offer(P128, dma, 128, 256, 4, F == 0 ? 1.02 : F == 1 ? 1.15 : 1.92);
+    offer(P192, dma && F < 2, 192, 256, 4, F == 0 ? 1.28 : 1.45);             // (16-bit operands do not fit its registers)
+    offer(P256, dma && (F == 0 || (F == 1 && p.kbytes % KROW == 0)), 256, 256, 5, F == 0 ? 1.57 : 1.95);
     if constexpr (OUT != OUT_E4M3) {
         if (best == ROWS16) return launch_rows<IN, OUT, 1, 3>(p, st);
         if (best == ROWS32) return launch_rows<IN, OUT, 2, 2>(p, st);
     }
-    if constexpr (F == 0)
-        if (best == R128) return launch_ring<IN, OUT, Ring<2, 2, 4, 4, 4, 1>>(p, st);
     if constexpr (F < 2) {
         if (best == P192) return launch_phased<IN, OUT, Phased<2, 4, 6, 4, 2>>(p, st);
         if (best == P256) return launch_phased<IN, OUT, Phased<2, 4, 8, 4, 2>>(p, st);
@@ -1051,6 +1067,7 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     switch (best) {
     case R32: return launch_ring<IN, OUT, Ring<1, 4, 2, 2, 3, 2>>(p, st);
     case R64: return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 3, 2>>(p, st);
+    case P128N: return launch_phased<IN, OUT, Phased<2, 4, 4, 2, 3>>(p, st);
     case P128: return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
     case ANY128: return launch_any<IN, OUT, Any<2, 4, 4, 2>>(p, st);
     default: return launch_any<IN, OUT, Any<1, 4, 2, 2>>(p, st);

@@ -193,6 +193,23 @@ def test_matmul_fp8(ops, m, n, k, scale, out):
             check(y, want, err, out, (m, n, k, relu))
 
 
+@pytest.mark.parametrize("m, n, k", [(2000, 2040, 400), (1571, 2048, 272), (4000, 2048, 656), (5000, 2040, 528), (8100, 2048, 16), (8100, 2000, 240), (8100, 2048, 1040), (3000, 1001, 419), (5000, 300, 63)])
+@pytest.mark.parametrize("form", ["bf16", E8, torch.float32])
+def test_products_whose_k_ends_inside_a_step(ops, m, n, k, form):
+    """in every tile size: what lies behind K in a wider tensor (NaN here) is not part of the sums"""
+    gap = 16 if k % 16 == 0 else 1
+    a, sa, b, sb, bias, offsets, index = grouped_inputs(ops, m, n, k, 1, form, [m], False, k)
+
+    def widened(t):
+        wide = torch.full((*t.shape[:-1], t.shape[-1] + gap), float("nan"), device="cuda").to(t.dtype)
+        wide.view(torch.int16 if form == "bf16" else torch.uint8)[..., :k] = t.view(torch.int16 if form == "bf16" else torch.uint8)
+        return wide[..., :k]
+    for out in (torch.float32, torch.bfloat16):
+        y = ops.matmul_grouped(widened(a), widened(b), offsets, a_scale=sa, b_scale=sb, bias=bias, out_dtype=out)
+        want, err = plain_grouped(a, sa, b, sb, bias, [m], None, False, form != "bf16" and out != torch.float32)
+        check(y, want, err, out, (m, n, k))
+
+
 def test_matmul_fp8_whole_numbers_are_exact(ops):
     """small whole numbers and powers of two: every sum is exact, so every lane, row and scale is where it belongs or the numbers differ"""
     g = gen(5)
