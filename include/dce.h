@@ -362,7 +362,7 @@ typedef enum dce_scale { DCE_SCALE_E8M0 = 0, DCE_SCALE_F32 = 1 } dce_scale;     
 /* x -> e4m3 and a power of two for every block: e = the smallest with max|x| <= 448 * 2^e, held inside [-126, 120]; q = x * 2^-e rounded once, ties to
  * even.  NaN and infinities become NaN and are left out of the maximum.  block_rows 1: activations, one matrix (batch 1), scale of row i and block t at
  * scale[t * ld_scale + i].  block_rows 128: weights, `batch` matrices, scale (batch, ceil(rows / 128), ceil(k / 128)) without gaps.  Any k; strides are
- * in values; x and q may not overlap. */
+ * in values; x and q may not overlap (refused where one matrix's do). */
 typedef struct dce_quantize_desc {
     const void* x;  int64_t ldx, x_batch;
     uint8_t*    q;  int64_t ldq, q_batch;
@@ -376,9 +376,11 @@ int  dce_quantize(int device_id, void* hip_stream, const dce_quantize_desc* d);
  * stays NaN); src(j) = index[j], or j where index is NULL; an index outside [0, a_rows) reads as a row of zeros.  offsets: groups + 1 numbers on the
  * DEVICE, never falling (NULL: one group of all m rows); they are held inside [0, m]; rows of y that no group covers stay as they were.  Operands bf16,
  * or e4m3 where a[i, k] stands for a * a_scale[(k / 128) * ld_a_scale + i] and b[g, c, k] for b * b_scale[g * b_scale_group + (c / 128) * ld_b_scale +
- * k / 128].  fp32 scales may be any finite numbers whose products are normal fp32 numbers or zero.  Sums are fp32; y is rounded once to y_type; e4m3
+ * k / 128].  fp32 scales may be any finite numbers whose products are normal fp32 numbers or zero;
+ * e8m0 scales any: an operand's value that is no normal fp32 number (448 * 2^120, 2^-9 * 2^-120) may count as infinite or as zero.  Sums are fp32; y is rounded once to y_type; e4m3
  * results take a power of two for every 128 columns of a row, y_scale[(c / 128) * ld_y_scale + j], in scale_type.  Any m, n and k (k = 0: the bias);
- * strides in values; 16-byte aligned rows run fastest.  y overlaps no operand.  The same call gives the same bits. */
+ * strides in values; 16-byte aligned rows run fastest.  y overlaps neither a nor b (refused
+ * where it is found to).  The same call gives the same bits. */
 typedef struct dce_matmul_desc {
     const void* a; int64_t lda; const void* a_scale; int64_t ld_a_scale;
     const void* b; int64_t ldb, b_group; const void* b_scale; int64_t ld_b_scale, b_scale_group;

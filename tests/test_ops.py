@@ -48,7 +48,7 @@ def _quantize(**kw):
 
 def _matmul(**kw):
     d = dict(a=4096, lda=256, a_scale=4096, ld_a_scale=4, b=4096, ldb=256, b_group=0, b_scale=4096, ld_b_scale=2, b_scale_group=0, bias=0, bias_group=0,
-             y=8192, ldy=64, y_scale=0, ld_y_scale=0, offsets=0, index=0, a_rows=4, m=4, n=64, k=256, groups=1, in_type=2, scale_type=0, out_type=0, relu=0, reserved=0)
+             y=1 << 24, ldy=64, y_scale=0, ld_y_scale=0, offsets=0, index=0, a_rows=4, m=4, n=64, k=256, groups=1, in_type=2, scale_type=0, out_type=0, relu=0, reserved=0)
     d.update(kw)
     return MATMUL.pack(*d.values())
 
@@ -57,7 +57,7 @@ def _matmul(**kw):
     (dict(x_type=2), b"x must be"), (dict(scale_type=2), b"scale type"), (dict(block_rows=64), b"a block has"), (dict(rows=-1), b"out of range"),
     (dict(k=1 << 25), b"out of range"), (dict(batch=2), b"one matrix"), (dict(ldx=255), b"stride"), (dict(ldq=255), b"stride"), (dict(x=0), b"NULL"), (dict(q=0), b"NULL"),
     (dict(scale=0), b"NULL"), (dict(x=4098), b"aligned"), (dict(scale=1026, scale_type=1), b"aligned"), (dict(ld_scale=3), b"ld_scale"),
-    (dict(batch=2, block_rows=128, q_batch=1000, rows=4), b"overlap")])
+    (dict(batch=2, block_rows=128, q_batch=1000, rows=4), b"overlap"), (dict(ldx=1 << 50), b"stride"), (dict(ldq=1 << 50), b"stride"), (dict(x=8192), b"overlap")])
 def test_quantize_refuses(lib, kw, word):
     assert lib.dce_quantize(0, None, _quantize(**kw)) == -1
     assert word in lib.dce_last_error(None)
@@ -70,7 +70,9 @@ def test_quantize_refuses(lib, kw, word):
     (dict(ldy=63), b"stride"), (dict(a=0), b"NULL"), (dict(b=0), b"NULL"), (dict(y=0), b"NULL"), (dict(a_scale=0), b"a_scale"), (dict(b_scale=0), b"a_scale"),
     (dict(ld_a_scale=3), b"scale"), (dict(ld_b_scale=1), b"scale"), (dict(out_type=2), b"y_scale"), (dict(out_type=2, y_scale=64, ld_y_scale=3), b"y_scale"),
     (dict(y=8194), b"aligned"), (dict(bias=4097), b"aligned"), (dict(in_type=1, a=4097), b"aligned"), (dict(scale_type=1, a_scale=4098), b"aligned"),
-    (dict(groups=2, offsets=64, b_group=-1), b"negative")])
+    (dict(groups=2, offsets=64, b_group=-1), b"negative"), (dict(groups=2, offsets=64, b_group=1 << 50), b"group stride"), (dict(lda=1 << 50), b"row stride"), (dict(ldb=1 << 50), b"row stride"),
+    (dict(ldy=1 << 50), b"row stride"), (dict(a=1 << 20, y=1 << 20), b"overlaps"), (dict(b=1 << 20, y=(1 << 20) + 64 * 256 - 4), b"overlaps"),
+    (dict(a=1 << 20, y=(1 << 20) - 4 * 64 * 4 + 4), b"overlaps"), (dict(groups=3, offsets=64, b=1 << 20, b_group=1 << 16, y=(1 << 20) + (2 << 16)), b"overlaps")])
 def test_matmul_refuses(lib, kw, word):
     assert lib.dce_matmul(0, None, _matmul(**kw)) == -1
     assert word in lib.dce_last_error(None)
@@ -82,6 +84,21 @@ def test_empty_calls_touch_nothing(lib):
     assert lib.dce_matmul(0, None, _matmul(m=0, a_rows=0, a=0, y=0, a_scale=0)) == 0
     assert lib.dce_matmul(0, None, _matmul(n=0, b=0, y=0)) == 0
     assert lib.dce_decide(0, None, None, 0, None, 0, None, None, None) == 0
+
+
+def test_overlap_is_found_where_it_is(lib):
+    """every place of y around a, against the bytes themselves: the same stride, and either one without gaps"""
+    if lib.dce_device_count() > 0:
+        pytest.skip("GPU present: the calls that are not refused would run")
+    base = 1 << 20
+    for lda, ldy, k, n, rows in ((24, 24, 8, 6, 3), (8, 24, 8, 6, 3), (24, 6, 8, 6, 3), (8, 6, 8, 6, 4), (20, 20, 8, 8, 1)):
+        a = {base + 2 * (i * lda + j) + u for i in range(rows) for j in range(k) for u in (0, 1)}
+        for d in range(-100, 101):
+            at = base + 2 * d
+            y = {at + 2 * (i * ldy + j) + u for i in range(rows) for j in range(n) for u in (0, 1)}
+            desc = _matmul(a=base, lda=lda, b=64, ldb=k, y=at, ldy=ldy, a_rows=rows, m=rows, n=n, k=k, in_type=1, out_type=1, a_scale=0, b_scale=0)
+            refused = lib.dce_matmul(0, None, desc) == -1
+            assert refused == bool(a & y), (lda, ldy, d, lib.dce_last_error(None))
 
 
 def test_null_descriptors_and_grouping_refusals(lib):
