@@ -4,7 +4,7 @@
 //
 // A power of two costs a floating-point format nothing: x * 2^-e is exact, so q carries the ONE rounding to 4 significant bits, and the matrix pipe
 // can apply the exponents itself.  NaN and infinities become NaN and do not set the scale.
-// Bound: memory, one read of x and one write of q.
+// Bound: memory, one read of x and one write of q: 32768 x 4736 bf16 83 us, 5.6 TB/s; one row 2.5 us, the launch.
 #include "block_ops.h"
 
 namespace dce {

@@ -1,6 +1,6 @@
 // torch_entries.cpp -- ops.py's entries on torch tensors: their checks, their results, one call of libdce's C ABI each (include/dce.h: dce_quantize,
 // dce_matmul, dce_group_rows, dce_decide).  A CPython extension module: the smallest of these products take the GPU 4 us, which checks and allocations
-// in Python took twice over (9.5 us a call for one row of 2048 x 4736; 5.9 here).  The library's functions come by address (bind): it is bound to the
+// in Python took twice over (9.5 us a call for one row of 2048 x 4736; 5.7 here).  The library's functions come by address (bind): it is bound to the
 // process's HIP runtime by _lib.py and not linked here.
 #include <Python.h>
 #include <torch/csrc/Exceptions.h>
