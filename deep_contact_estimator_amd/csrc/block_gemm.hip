@@ -357,6 +357,32 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
     }
 }
 
+// The sums of the groups that share K, group 0's first; the other group is done then
+template <int OUT, class T>
+__device__ __forceinline__ bool gather_groups(f32x4 (&acc)[T::MT][T::NT], char* smem, int kg, int wave, int lane)
+{
+    if constexpr (T::KG == 2) {
+        constexpr int B = T::MT * T::NT;
+        static_assert(T::WAVES * B * 1024 <= T::LDS, "LDS");
+        f32x4* const sums = reinterpret_cast<f32x4*>(smem) + wave * B * 64 + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int i = 0; i < B; ++i) sums[i * 64] = acc[i / T::NT][i % T::NT];
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int i = 0; i < B; ++i) acc[i / T::NT][i % T::NT] += sums[i * 64];
+        }
+        __syncthreads();
+        if (kg == 1) {
+            if (OUT == OUT_E4M3) __syncthreads();                             // (store_tile's)
+            return false;
+        }
+    }
+    return true;
+}
+
 template <int IN, int OUT, class T>
 __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs p)
 {
@@ -510,32 +536,17 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
 #pragma unroll
     for (int i = 0; i < MT; ++i) spoil<IN, EXACT, NT>(acc[i], bad[i]);
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
-    if constexpr (KG == 2) {
-        f32x4* const sums = reinterpret_cast<f32x4*>(smem) + wave * MT * NT * 64 + lane;
-        if (kg == 1) {
-#pragma unroll
-            for (int i = 0; i < MT * NT; ++i) sums[i * 64] = acc[i / NT][i % NT];
-        }
-        __syncthreads();
-        if (kg == 0) {
-#pragma unroll
-            for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += sums[i * 64];
-        }
-        __syncthreads();
-        if (kg == 1) {
-            if (OUT == OUT_E4M3) __syncthreads();                             // (store_tile's)
-            return;
-        }
-    }
+    if (!gather_groups<OUT, T>(acc, smem, kg, wave, lane)) return;
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
 // ---- the kernel for operands at any address: panels come through registers as whole words, two steps ahead, and are shifted to their bytes on the way to
-//      LDS (16-byte loads that do not start at a word take longer: 733 rows of 1001 x 1419 to fp32 22.6 us with them and a last step byte by byte, 14.5
-//      so).  A lane's last word is its neighbour's first.
-template <int WM_, int WN_, int MT_, int NT_> struct Any {
-    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr int AT_ONCE = THREADS / 8, CH = (BM + BN) / AT_ONCE, LDS = 2 * (BM + BN) * KROW;   // rows that all threads bring together; 16-byte chunks a thread and step
+//      LDS (a lane's last word is its neighbour's first).  Bound: the shifts and a wave's latencies, so the small tile's steps are dealt out to two groups
+//      of waves as the ring's are.  733 rows of 1001 x 1419 to fp32: 16-byte loads from any address and a last step byte by byte 22.6 us, whole words
+//      14.5, two groups 12.9.
+template <int WM_, int WN_, int MT_, int NT_, int KG_> struct Any {
+    static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, KG = KG_, BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES * KG;
+    static constexpr int AT_ONCE = WAVES * 8, CH = (BM + BN) / AT_ONCE, LDS = KG * 2 * (BM + BN) * KROW;   // rows that a group brings together; 16-byte chunks a thread and step
     static_assert(BN == BLK && BM % AT_ONCE == 0 && BN % AT_ONCE == 0, "tile");
 };
 
@@ -548,14 +559,15 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
     Place at;
     if (!find_tile(p, BM, at)) return;
     const int g = at.g, first = at.first, end = at.end, tn = at.tn;
-    const int n0 = tn * BN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int n0 = tn * BN, lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % T::WAVES, kg = all / T::WAVES, r = lane & 15, q = lane >> 4;
     const int wm = (wave / T::WN) * MT * 16, wn = (wave % T::WN) * NT * 16;
-    const int steps = p.a_rows ? (p.kbytes + KROW - 1) / KROW : 0;
+    const int total = p.a_rows ? (p.kbytes + KROW - 1) / KROW : 0, rounds = (total + T::KG - 1) / T::KG;    // this group's steps: kg, kg + KG, ..; a round: one of every group
+    const int steps = kg < total ? (total - kg + T::KG - 1) / T::KG : 0, t8 = wave * 8 + (lane >> 3);
 
     const char* row[CH];                                                      // (rows without a source and columns behind the last: any, not stored or taken out at the end)
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-        const int lr = (int)(threadIdx.x >> 3) + T::AT_ONCE * i;
+        const int lr = t8 + T::AT_ONCE * i;
         if (lr < BM) { const long long s = source_row(p, first + lr, end); row[i] = p.a + (s < 0 ? 0 : s) * p.a_row; }
         else { const int c = n0 + lr - BM; row[i] = p.b + g * p.b_group + (long long)(c < p.n ? c : p.n - 1) * p.b_row; }
     }
@@ -565,7 +577,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
     for (int i = 0; i < MT; ++i) { const long long s = source_row(p, first + wm + i * 16 + r, end); mine[i] = s < 0 ? 0 : s; }
     const long long sb0 = g * p.sb_group + (long long)tn * p.sb_row;
     struct Step { i32x4 v[CH]; int next[CH]; unsigned sw, sx[MT]; } even, odd;
-    auto fetch = [&](int s, Step& f) {
+    auto fetch = [&](int round, Step& f) {
+        const int s = round * T::KG + kg;
         const int from = s * KROW + c8 * 16;
         if ((s + 1) * KROW <= p.kbytes) {
 #pragma unroll
@@ -602,20 +615,22 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    auto step = [&](int s, Step& f) {
-        char* const lds = smem + (s & 1) * (BM + BN) * KROW;                  // (last read two steps ago: a barrier lies between)
+    auto step = [&](int round, Step& f) {
+        const int s = round * T::KG + kg;
+        char* const lds = smem + (kg * 2 + (round & 1)) * (BM + BN) * KROW;   // (last read two rounds ago: a barrier lies between)
+        if (round >= steps) { __syncthreads(); return; }                      // (every group comes to every barrier)
         const int left = p.kbytes - s * KROW - c8 * 16;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int over = __builtin_amdgcn_update_dpp(0, f.v[i][0], 0x101, 0xf, 0xf, false);          // the next lane's first word
             i32x4 v = shift_words(f.v[i], c8 == 7 ? f.next[i] : over, (unsigned)reinterpret_cast<uintptr_t>(row[i]) & 3);
             if ((s + 1) * KROW > p.kbytes) v = cut_bytes(v, left);
-            *reinterpret_cast<i32x4*>(lds + slot_of((int)(threadIdx.x >> 3) + T::AT_ONCE * i, c8)) = v;
+            *reinterpret_cast<i32x4*>(lds + slot_of(t8 + T::AT_ONCE * i, c8)) = v;
         }
         unsigned sw = f.sw, sx[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) sx[i] = f.sx[i];
-        if (s + 2 < steps) fetch(s + 2, f);
+        if (round + 2 < steps) fetch(round + 2, f);
         __syncthreads();
         Frag<IN, EXACT> w[NT];
 #pragma unroll
@@ -636,13 +651,14 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
     for (int i = 0; i < CH; ++i) even.next[i] = odd.next[i] = 0;
     if (steps > 0) fetch(0, even);
     if (steps > 1) fetch(1, odd);
-    for (int s = 0; s < steps; s += 2) {
+    for (int s = 0; s < rounds; s += 2) {
         step(s, even);
-        if (s + 1 < steps) step(s + 1, odd);
+        if (s + 1 < rounds) step(s + 1, odd);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) spoil<IN, EXACT, NT>(acc[i], bad[i]);
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
+    if (!gather_groups<OUT, T>(acc, smem, kg, wave, lane)) return;
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
 }
 
@@ -965,7 +981,9 @@ hipError_t launch_any(ProductArgs p, hipStream_t st)
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long grid = (row_tiles(p, T::BM) * p.tiles_n + 7) / 8 * 8;
     if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
-    static_assert(T::LDS <= 64 * 1024, "LDS");
+    static std::atomic<unsigned long long> devices{0};
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(product_any_kernel<IN, OUT, T>), T::LDS, devices);
+    if (e != hipSuccess) return e;
     product_any_kernel<IN, OUT, T><<<(unsigned)grid, T::THREADS, T::LDS, st>>>(p);
     return hipGetLastError();
 }
@@ -1021,8 +1039,7 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 //     8192                                                                           81.3        92.5        66.9
 //    32768                                       941.9      626.2       409         309.6       301.7       263.2
 //
-// Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 12.1 | 17.2, 1500 16.1 | 17.6, 3000 23.7 | 19.5, 20000 118 | 93;
-// 4096 166.9 | 99.5.
+// Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 11.0 | 17.2, 3000 23.7 | 19.3, 20000 118 | 93; 4096 167 | 99.
 //
 // Folded block sums (fp32 scales) take 1.05 .. 1.2 times as long, 16-bit operands from e4m3 (fp32 results) 1.4 times in the rings and 1.6 .. 1.9 in the
 // large tiles (1571 rows 41 us, 32768 490 with e8m0 scales and 529 with fp32 ones), bf16 operands over the same K twice, since a step of K is 64 of theirs.
@@ -1032,7 +1049,7 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
     constexpr bool EXACT = OUT == OUT_F32;
     constexpr int F = IN != IN_BF16 && EXACT ? 2 : FOLDS<IN, EXACT> ? 1 : 0;                 // scales for the matrix instruction (or none) | block sums folded | e4m3 as fp16
-    if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT, Any<1, 4, 2, 2>>(p, st);
+    if (p.kbytes == 0 || p.a_rows == 0) return launch_any<IN, OUT, Any<1, 4, 2, 2, 2>>(p, st);
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | (uintptr_t)p.a_row | (uintptr_t)p.b_row | (uintptr_t)p.b_group | (uintptr_t)p.kbytes) & 15) == 0;
     const bool near = p.sb_row < (1ll << 29) && p.a_rows * p.a_row < (1ll << 32) && p.n * p.b_row < (1ll << 32);      // the ring's and the phased kernel's 32-bit offsets
     const bool dma = aligned && near;
@@ -1069,8 +1086,8 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     case R64: return launch_ring<IN, OUT, Ring<2, 2, 2, 4, 3, 2>>(p, st);
     case P128N: return launch_phased<IN, OUT, Phased<2, 4, 4, 2, 3>>(p, st);
     case P128: return launch_phased<IN, OUT, Phased<2, 4, 4, 4, 3>>(p, st);
-    case ANY128: return launch_any<IN, OUT, Any<2, 4, 4, 2>>(p, st);
-    default: return launch_any<IN, OUT, Any<1, 4, 2, 2>>(p, st);
+    case ANY128: return launch_any<IN, OUT, Any<2, 4, 4, 2, 1>>(p, st);
+    default: return launch_any<IN, OUT, Any<1, 4, 2, 2, 2>>(p, st);
     }
 }
 
