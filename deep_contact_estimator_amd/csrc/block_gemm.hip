@@ -250,9 +250,18 @@ template <int WM_, int WN_, int MT_, int NT_, int NBUF_, int KG_> struct Ring {
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES * KG;
     static constexpr int PANELS = (BM + BN) * KROW, PIECES = PANELS / 1024 / WAVES;   // a piece: eight rows, one instruction
     static constexpr int SA = (BM + 63) / 64, SLOT = (SA + 1) * 256, BUF = PANELS + SLOT;  // waves that bring the rows' scales; a word a row, then the columns'
-    static constexpr int LDS = KG * NBUF * BUF;
+    static constexpr int BIAS = KG * NBUF * BUF, LDS = BIAS + BN * 4;
     static_assert(PANELS % (1024 * WAVES) == 0 && BM % 8 == 0 && BN == BLK && LDS <= 160 * 1024 && SA < WAVES && WAVES == 4, "tile");
 };
+
+// The tile's bias -> LDS, asked for first and there with the first panels (the epilogue would wait for it once more)
+template <class T>
+__device__ __forceinline__ void bring_bias(const ProductArgs& p, const char* smem, int g, int n0, int wave, int lane)
+{
+    if (!p.bias || wave * 64 >= T::BN) return;
+    const int c = n0 + wave * 64 + lane;
+    dma4s(reinterpret_cast<const char*>(p.bias + g * p.bias_group), (unsigned)(c < p.n ? c : p.n - 1) * 4, lds_addr(smem) + T::BIAS + wave * 256);
+}
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
 // sixteen rows at a time round in its own corner of LDS (a lane holds four columns of a row, a store takes neighbouring lanes along a row).  Rows of y that
@@ -264,15 +273,10 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
     const int r = lane & 15, q = lane >> 4, wm = (wave / T::WN) * T::MT * 16, wn = (wave % T::WN) * T::NT * 16;
     float* const most = reinterpret_cast<float*>(smem);                       // [wave column][row]
     char* const turn = smem + (OUT == OUT_E4M3 ? T::WN * T::BM * 4 : 0) + wave * 16 * PITCH;
-    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH <= T::LDS, "LDS");
+    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH <= T::BIAS, "LDS");
     f32x4 bias[T::NT];
 #pragma unroll
-    for (int u = 0; u < T::NT; ++u)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int c = n0 + wn + u * 16 + q * 4 + v;
-            bias[u][v] = p.bias && c < p.n ? p.bias[g * p.bias_group + c] : 0.f;
-        }
+    for (int u = 0; u < T::NT; ++u) bias[u] = p.bias ? *reinterpret_cast<const f32x4*>(smem + T::BIAS + (wn + u * 16 + q * 4) * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
     float top[T::MT];
 #pragma unroll
     for (int i = 0; i < T::MT; ++i) {
@@ -363,7 +367,7 @@ __device__ __forceinline__ bool gather_groups(f32x4 (&acc)[T::MT][T::NT], char* 
 {
     if constexpr (T::KG == 2) {
         constexpr int B = T::MT * T::NT;
-        static_assert(T::WAVES * B * 1024 <= T::LDS, "LDS");
+        static_assert(T::WAVES * B * 1024 <= T::BIAS, "LDS");
         f32x4* const sums = reinterpret_cast<f32x4*>(smem) + wave * B * 64 + lane;
         if (kg == 1) {
 #pragma unroll
@@ -464,6 +468,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bring_bias<T>(p, smem, g, n0, all, lane);
 #pragma unroll
     for (int s = 0; s < NBUF; ++s) if (s < steps) bring(s, 0, T::PIECES);
     int buf = 0;
@@ -546,7 +551,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_ring_kernel(ProductArgs
 //      14.5, two groups 12.9.
 template <int WM_, int WN_, int MT_, int NT_, int KG_> struct Any {
     static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, KG = KG_, BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES * KG;
-    static constexpr int AT_ONCE = WAVES * 8, CH = (BM + BN) / AT_ONCE, LDS = KG * 2 * (BM + BN) * KROW;   // rows that a group brings together; 16-byte chunks a thread and step
+    static constexpr int AT_ONCE = WAVES * 8, CH = (BM + BN) / AT_ONCE, BIAS = KG * 2 * (BM + BN) * KROW, LDS = BIAS + BN * 4;   // rows that a group brings together; 16-byte chunks a thread and step
     static_assert(BN == BLK && BM % AT_ONCE == 0 && BN % AT_ONCE == 0, "tile");
 };
 
@@ -649,6 +654,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
     for (int i = 0; i < MT; ++i) even.sx[i] = odd.sx[i] = 0;
 #pragma unroll
     for (int i = 0; i < CH; ++i) even.next[i] = odd.next[i] = 0;
+    bring_bias<T>(p, smem, g, n0, all, lane);
     if (steps > 0) fetch(0, even);
     if (steps > 1) fetch(1, odd);
     for (int s = 0; s < rounds; s += 2) {
@@ -657,6 +663,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) spoil<IN, EXACT, NT>(acc[i], bad[i]);
+    wait_all_but<0>();
     __syncthreads();                                                          // the panels have been read: LDS is the epilogue's
     if (!gather_groups<OUT, T>(acc, smem, kg, wave, lane)) return;
     store_tile<IN, OUT, T>(p, acc, smem, g, first, end, n0, wave, lane);
@@ -680,7 +687,7 @@ template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BUF = (BM + BN) * KROW, PA = BM / 64, PB = BN / 64;   // pieces of eight rows a wave brings: of its group's rows, of the weights
     static constexpr int SLOT = (BM + 64) * 4;                                // a step's scales: the rows', the column blocks'
-    static constexpr int LDS = NBUF * BUF + 4 * SLOT;
+    static constexpr int BIAS = NBUF * BUF + 4 * SLOT, LDS = BIAS + BN * 4;
     template <int IN> static constexpr bool TAIL = !(MT == 8 && IN == IN_F8_F32);   // (no register left where block sums are folded)
     static_assert(WM == 2 && WN == 4 && BN / BLK <= 64 && (NBUF == 2 || NBUF == 3), "two groups of four waves");
 };
@@ -775,6 +782,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bring_bias<T>(p, smem, g, n0, wave, lane);
     bring(0, 0, 0, ALL);
     if (steps > 1) { bring(1, 1, 0, ALL); wait_all_but<ALL>(); }
     else { wait_all_but<0>(); clear_tail(0); }
