@@ -25,7 +25,7 @@ struct Place { int g, first, end, tn; };      // a tile: its group, its first ro
 
 // The tile of this workgroup.  Row tiles are counted group by group (offsets are held inside [0, m] whatever they say) and only here: the host knows no
 // more than a bound.  Workgroups go round the eight XCDs, so workgroup 8 i + x takes the i-th tile of the x-th eighth of those that there are: neighbours
-// share an L2, columns first.  64 groups a step, tiles counted by a scan over the lanes; every wave does it for itself.
+// share an L2: bands of eight column tiles, columns first (32 CUs: 4 x 8 tiles, 12 panels a step from beyond the L2 and 52 out of it).  64 groups a step, tiles counted by a scan over the lanes; every wave does it for itself.
 __device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, Place& at)
 {
     const int lane = threadIdx.x & 63;
@@ -43,8 +43,9 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, Place& a
     else for (int base = 0; base < p.groups; base += 64) total += scan(base);
     const unsigned all = (unsigned)total * (unsigned)p.tiles_n, per = (all + 7) >> 3, slot = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + slot;
     if (slot >= per || id >= all) return false;
-    const int t = (int)(id / (unsigned)p.tiles_n);
-    at.tn = (int)(id % (unsigned)p.tiles_n);
+    const unsigned band = id / ((unsigned)total * 8), wide = p.tiles_n - band * 8 < 8 ? p.tiles_n - band * 8 : 8, in = id - band * total * 8;
+    const int t = (int)(in / wide);
+    at.tn = (int)(band * 8 + in % wide);
     if (!p.offsets) { at.g = 0; at.first = t * bm; at.end = p.m; return true; }
     int before = 0;
     for (int base = 0; base < p.groups; base += 64) {
@@ -762,7 +763,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             *reinterpret_cast<i32x4*>(smem + buf * T::BUF + piece * 1024 + lane * 16) = i32x4{0, 0, 0, 0};
         }
     };
-    constexpr int ALL = PB + PS + PA;
+    constexpr int ALL = PB + PS + PA, FIRST = NBUF == 2 ? PB + PS + XG / 2 : ALL;   // (two buffers: rows that the first reads of a step take, XG / 2 pieces a wave, are free before the rest)
     auto phase_end = [&] {                                                    // (matrix instructions touch no memory: the scheduling barriers keep them in their phase)
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -784,21 +785,27 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
     }
     bring_bias<T>(p, smem, g, n0, wave, lane);
     bring(0, 0, 0, ALL);
-    if (steps > 1) { bring(1, 1, 0, ALL); wait_all_but<ALL>(); }
+    if (steps > 1) { bring(1, 1, 0, FIRST); wait_all_but<FIRST>(); }
     else { wait_all_but<0>(); clear_tail(0); }
     phase_end();
     if (grp == 1) {
         if (NBUF == 3 && steps > 2) bring(2, 2, 0, ALL);
         phase_end();
     }
-    int buf = 0;                                                              // of step s; that of s + 2 (two buffers: the same)
+    int buf = 0;                                                              // of step s
     for (int s = 0; s < steps; ++s) {
-        const int buf2 = NBUF == 2 ? buf : buf == 0 ? 2 : buf - 1;
+        const int buf1 = buf == NBUF - 1 ? 0 : buf + 1, buf2 = buf1 == NBUF - 1 ? 0 : buf1 + 1;      // of the steps behind it
         const char* const xa = smem + buf * T::BUF;
         const char* const wa = xa + BM * KROW;
         const unsigned* const scales = reinterpret_cast<const unsigned*>(smem + NBUF * T::BUF + (s & 3) * T::SLOT);
-        const bool more = s + 2 < steps;
-        const int buf1 = buf == NBUF - 1 ? 0 : buf + 1;
+        const bool more1 = s + 1 < steps, more2 = s + 2 < steps;
+        // what the next reads but one phase need is there: the last two sets of requests are not part of it
+        auto landed = [&](int h) {
+            if (h < H - 1 ? !more1 : !more2) wait_all_but<0>();
+            else if (h == H - 1 && XG % 2) wait_all_but<FIRST>();             // (a piece holds rows of both reads)
+            else wait_all_but<ALL>();
+            if (h == H - 1 && s + 2 == steps) clear_tail(buf1);
+        };
         Frag<IN, EXACT> w[NT];
         unsigned sw = 0;
 #pragma unroll
@@ -817,12 +824,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
                 if (PS) sv[i] = scales[row];
                 x[i].set(chunk(xa, row, q), chunk(xa, row, q + 4), PS ? sv[i] : 0);
             }
-            if (h == H - 1 && grp == 1) {                                     // step s + 1 is there but for what was asked for after it
-                if (!more) wait_all_but<0>();
-                else if (NBUF == 3) wait_all_but<ALL>();
-                else wait_all_but<PB>();
-                if (s + 2 == steps) clear_tail(buf1);
-            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (NBUF == 3) {}
+            else if (h == H - 1) { if (more2) bring(s + 2, buf, 0, FIRST); }
+            else if (more1) bring(s + 1, buf1, FIRST, ALL);
+            if (grp == 1) landed(h);
             phase_end();
             // ---- M
             __builtin_amdgcn_s_setprio(1);
@@ -832,24 +838,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             for (int i = 0; i < XG; ++i) {
                 if (PS) sc[i & 1].set(sw, sv[i], bad[h * XG + i]);
                 mfma_row<IN, EXACT, NT>(acc[h * XG + i], part[i & 1], w, x[i], sc[i & 1]);
-                // requests between the instructions, a few behind each row: the pipe is busy while they are issued
-                int next = s + 2;
-                bool ask;
-                if constexpr (NBUF == 2) {
-                    if (grp == 0) { next = h == 0 ? s + 1 : s + 2; ask = next < steps && (h > 0 || s > 0); }
-                    else ask = more;
-                } else {
-                    next = s + 2 + grp;
-                    ask = next < steps && h == (grp == 0 ? 0 : H - 1);
-                }
-                if (ask && i < XG - 1) {
-                    const int to = NBUF == 2 ? next & 1 : grp == 0 ? buf2 : buf;
+                if (NBUF == 3 && s + 2 + grp < steps && i < XG - 1) {         // requests between the instructions, some behind each row: the pipe is busy while they are issued
                     if constexpr (FOLDS<IN, EXACT>) pin(part[i & 1]);
                     else pin(acc[h * XG + i]);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (NBUF == 3) bring(next, to, i * ALL / (XG - 1), (i + 1) * ALL / (XG - 1));
-                    else if (h == 0) bring(next, to, i * PB / (XG - 1), (i + 1) * PB / (XG - 1));
-                    else bring(next, to, PB + i * (PS + PA) / (XG - 1), PB + (i + 1) * (PS + PA) / (XG - 1));
+                    bring(s + 2 + grp, grp ? buf : buf2, i * ALL / (XG - 1), (i + 1) * ALL / (XG - 1));
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (i > 0) fold_row<IN, EXACT, NT>(acc[h * XG + i - 1], part[(i - 1) & 1], sc[(i - 1) & 1]);
@@ -858,12 +851,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_phased_kernel(ProductAr
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int i = 0; i < XG; ++i) pin(acc[h * XG + i]);
-            if (h == H - 1 && grp == 0) {
-                if (!more) wait_all_but<0>();
-                else if (NBUF == 3) wait_all_but<ALL>();
-                else wait_all_but<PA + PS>();
-                if (s + 2 == steps) clear_tail(buf1);
-            }
+            if (grp == 0) landed(h);
             phase_end();
         }
         buf = buf1;
@@ -1067,7 +1055,7 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     double least = 0;
     auto offer = [&](int kernel, bool can, int bm, int bn, double edge, double step) {
         if (!can) return;
-        const double rows = p.offsets ? (double)p.m / bm + 0.5 * (p.groups < p.m ? p.groups : p.m) : (double)((p.m + bm - 1) / bm);   // (a group's last tile is half full)
+        const double rows = p.groups > 1 ? (double)p.m / bm + 0.5 * (p.groups < p.m ? p.groups : p.m) : (double)((p.m + bm - 1) / bm);   // (a group's last tile is half full)
         const double us = 2 + ceil(rows * ((p.n + bn - 1) / bn) / 256) * (edge + steps * step);
         if (best < 0 || us < least) { best = kernel; least = us; }
     };
