@@ -672,17 +672,19 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
 
 // ---- the kernel for chip-filling products (operands within 4 GB): eight waves in two groups that are a phase apart.
 //
-// Waves w and w + 4 share a SIMD.  While one group's phase is its matrix instructions, the other group's is reads of fragments from LDS and waits: the
-// matrix pipe passes from one group to the other without a pause, and no wave waits for LDS with the pipe idle.  A step of group 0 is L0 M0 .. (of
-// H = MT / XG pairs; L: XG rows of blocks read, M: multiplied; L0 reads all of the weights' fragments too), from phase 2H s on; group 1 runs the same
-// one phase later; a barrier ends every phase.
+// Waves w and w + 4 share a SIMD.  While one group's phase is its matrix instructions, the other group's is reads of fragments from LDS, requests and
+// waits: the matrix pipe passes from one group to the other, and no wave waits for LDS with the pipe idle.  A step of group 0 is L0 M0 .. (of H = MT / XG
+// pairs; L: XG rows of blocks read, M: multiplied; L0 reads all of the weights' fragments too), from phase 2H s on; group 1 runs the same one phase
+// later; a barrier ends every phase.
 //
-// 64 KB a step and CU are 1 us of what L2 gives to all CUs at once (measured, 17 TB/s) and another half before the first of them is there, against 0.9 us
-// of matrix instructions: panels have to be asked for more than a step ahead.  256 x 256 tiles leave room for two buffers, so each part of a panel is
-// asked for once its buffer has been read for the last time, a quarter of a step's requests (they take the CU 1150 cycles in all) in every phase: of step
-// s + 2, group 1's half of the weights at phase 4s + 2, group 0's rows at 4s + 3, group 1's at 4s + 4, group 0's half of the weights at 4s + 5.  Smaller
-// tiles have three buffers: step s + 2 at phase 2H s + 1, by group 1 at 2H s.  All of it between matrix instructions.  Scales come the same way, a word
-// a row.
+// Panels (64 KB a step of 256 x 256) have to be asked for more than a step ahead.  Two buffers: each part of a panel once its buffer has been read for the
+// last time, in L phases behind the reads -- of step s + 2 the weights and the first rows in the last L of step s, the other rows (then read themselves) in
+// L0 of step s + 1; five phases or more lie between a request and its use.  Three buffers (smaller tiles, whose L phases are longer than their M phases):
+// between matrix instructions, step s + 2 at phase 2H s + 1, by group 1 at 2H s.  Scales come the same way, a word a row.
+//
+// What bounds it, at 8192 x 2048 over long K: 1.10 us a step of 256 x 256 (zeros: the clock at its highest), with or without its requests, 0.87 of them
+// matrix instructions and the rest the phases' barriers; 1.39 with random operands, where the power limit sets the clock (a library product of one scale
+// for all: 0.86 and 1.18).  Requests between matrix instructions took 1.45 and 1.7 there.  8192^3: e4m3 2680 TFLOP/s, bf16 1390.
 template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
     static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
@@ -1025,21 +1027,20 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 //
 //   rows   e4m3 to bf16:   16 / 32 at a time   32 x 128   64 x 128   128 x 128   128 x 256   192 x 256   256 x 256
 //        1                       5.5 /  6.2       14.3       16.6
-//       32                       7.3 /  9.5       14.6       16.9
-//      128                      25.8 / 18.5       15.6       17.3                    31.5        41.1        50.5
-//     1024                                        32.3       20.9        24.6        33.5        44.8        52.7
-//     1571                                                   31.3        28.0
-//     2048                                        59.9       38.5        30.1        35.3        46.5        53.9
-//     4096                                       114.8       76.9        53.9        46.3        50.7        56.7
-//     5000                                       141.0       90.9                    69.5        53.2        57.5
-//     8192                                                                           81.3        92.5        66.9
-//    32768                                       941.9      626.2       409         309.6       301.7       263.2
+//       32                       7.3 /  9.5       14.5       16.8
+//      128                      25.8 / 18.5       15.6       17.3
+//     1024                                        30.3       19.8        26.2        32.5        47.7        53.6
+//     2048                                        55.3       36.5        31.2        34.9        49.4        55.2
+//     4096                                                               57.1        46.2        52.9        57.5
+//     5000                                                               75.2        67.8        55.2        58.4
+//     8192                                                              104.5        78.6        95.7        71.9
+//    32768                                       941.9      626.2       383.1       303.2       300.4       259.6
 //
 // Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 11.0 | 17.2, 3000 23.7 | 19.3, 20000 118 | 93; 4096 167 | 99.
 //
-// Folded block sums (fp32 scales) take 1.05 .. 1.2 times as long, 16-bit operands from e4m3 (fp32 results) 1.4 times in the rings and 1.6 .. 1.9 in the
-// large tiles (1571 rows 41 us, 32768 490 with e8m0 scales and 529 with fp32 ones), bf16 operands over the same K twice, since a step of K is 64 of theirs.
-// A K that ends inside a step costs up to 5 % (4720 instead of 4736: 4096 rows 47.4 us, not 42.5 .. 46).
+// Folded block sums (fp32 scales) take 1.02 .. 1.2 times as long (32768 rows 305), 16-bit operands from e4m3 (fp32 results) 1.35 times in the rings and
+// 1.4 .. 1.9 in the large tiles (2048 rows 43.3, 32768 499 with e8m0 scales and 542 with fp32 ones), bf16 operands over the same K twice, since a step of
+// K is 64 of theirs (4096 rows 78.7 in 128 x 256 tiles, 32768 478 in 256 x 256).  A K that ends inside a step costs up to 5 %.
 template <int IN, int OUT>
 hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {
@@ -1063,12 +1064,12 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     offer(ROWS32, OUT != OUT_E4M3, 32, 16, 1.5, aligned ? 0.17 : 0.25);
     offer(ANY, !dma, 32, 128, 2, F ? 0.6 : 0.5);                              // (several at once on a CU)
     offer(ANY128, !dma, 128, 128, 3, F ? 1.65 : 1.2);
-    offer(R32, dma, 32, 128, 2, F == 0 ? 0.35 : F == 1 ? 0.37 : 0.50);
-    offer(R64, dma, 64, 128, 2, F == 0 ? 0.44 : F == 1 ? 0.46 : 0.70);
-    offer(P128N, dma, 128, 128, 3, F == 0 ? 0.68 : F == 1 ? 0.70 : 1.22);
-    offer(P128, dma, 128, 256, 4, F == 0 ? 1.02 : F == 1 ? 1.15 : 1.92);
-    offer(P192, dma && F < 2, 192, 256, 4, F == 0 ? 1.28 : 1.45);             // (16-bit operands do not fit its registers)
-    offer(P256, dma && (F == 0 || (F == 1 && p.kbytes % KROW == 0)), 256, 256, 5, F == 0 ? 1.57 : 1.95);
+    offer(R32, dma, 32, 128, 2, F == 0 ? 0.34 : F == 1 ? 0.36 : 0.50);
+    offer(R64, dma, 64, 128, 2, F == 0 ? 0.42 : F == 1 ? 0.45 : 0.69);
+    offer(P128N, dma, 128, 128, 3, F == 0 ? 0.68 : F == 1 ? 0.69 : 1.06);
+    offer(P128, dma, 128, 256, 4, F == 0 ? 1.03 : F == 1 ? 1.13 : 1.75);
+    offer(P192, dma && F < 2, 192, 256, 4, F == 0 ? 1.30 : 1.44);             // (16-bit operands do not fit its registers)
+    offer(P256, dma && (F == 0 || (F == 1 && p.kbytes % KROW == 0)), 256, 256, 5, F == 0 ? 1.60 : 1.90);
     if constexpr (OUT != OUT_E4M3) {
         if (best == ROWS16) return launch_rows<IN, OUT, 1, 3>(p, st);
         if (best == ROWS32) return launch_rows<IN, OUT, 2, 2>(p, st);
