@@ -264,6 +264,68 @@ __device__ __forceinline__ void bring_bias(const ProductArgs& p, const char* sme
     dma4s(reinterpret_cast<const char*>(p.bias + g * p.bias_group), (unsigned)(c < p.n ? c : p.n - 1) * 4, lds_addr(smem) + T::BIAS + wave * 256);
 }
 
+// ---- the scale of e4m3 results.  Its exponent hangs on which side of 448 * 2^e a block's largest value lies, and the sums of the 8-bit matrix instruction are
+// good to 2^-16 of them, not to fp32: of 65536 blocks one or two would come out on the other side.  So where a largest value is within 2^-11 of such a
+// border (one block in 600) that value is summed once more, in fp32, by one wave: 3 us where a tile has such a block (2048 rows of 2048 x 4736 30.5 ->
+// 33.8 us, 4096 43.9, 32768 257 -> 271).
+struct Doubts {                                                               // in LDS
+    static constexpr int MAX = 256;                                           // more in one tile (all values alike): it keeps its sums
+    int count, where[MAX];                                                    // row << 16 | column in the tile
+    int exact[512];                                                           // a block's largest value, summed again
+};
+__device__ __forceinline__ bool in_doubt(float most)
+{
+    const int m = (int)(__float_as_uint(most) & 0x7fffffu) - 0x600000;        // (448 = 1.75 * 2^8)
+    return m > -7168 && m < 7168;
+}
+template <int IN>
+__device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, int g, int c, int lane)
+{
+    const char* const a = p.a + src * p.a_row;
+    const char* const b = p.b + g * p.b_group + (long long)c * p.b_row;
+    const long long sb0 = g * p.sb_group + (long long)(c / BLK) * p.sb_row;
+    float sum = 0.f;
+    auto add = [&](i32x4 x, i32x4 w, float s) {
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            part = fmaf(__builtin_amdgcn_cvt_f32_fp8(x[i], 0), __builtin_amdgcn_cvt_f32_fp8(w[i], 0), part);
+            part = fmaf(__builtin_amdgcn_cvt_f32_fp8(x[i], 1), __builtin_amdgcn_cvt_f32_fp8(w[i], 1), part);
+            part = fmaf(__builtin_amdgcn_cvt_f32_fp8(x[i], 2), __builtin_amdgcn_cvt_f32_fp8(w[i], 2), part);
+            part = fmaf(__builtin_amdgcn_cvt_f32_fp8(x[i], 3), __builtin_amdgcn_cvt_f32_fp8(w[i], 3), part);
+        }
+        sum = fmaf(part, s, sum);
+    };
+    auto scale = [&](int t) {
+        if constexpr (IN == IN_F8_F32) return static_cast<const float*>(p.sa)[t * p.sa_block + src] * static_cast<const float*>(p.sb)[sb0 + t];
+        else return ldexpf(1.f, (int)static_cast<const unsigned char*>(p.sa)[t * p.sa_block + src] + (int)static_cast<const unsigned char*>(p.sb)[sb0 + t] - 254);
+    };
+    int at = lane * 16;
+#pragma unroll 1
+    for (; at + 3 * 1024 + 16 <= p.kbytes; at += 4 * 1024) {                  // (a wave's latency is what this costs: four steps' loads at once)
+        i32x4 x[4], w[4];
+        float s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) { x[u] = load16(a + at + u * 1024); w[u] = load16(b + at + u * 1024); s[u] = scale((at + u * 1024) / BLK); }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) add(x[u], w[u], s[u]);
+    }
+#pragma unroll 1
+    for (; at < p.kbytes; at += 1024) add(load16_tail(a, at, p.kbytes), load16_tail(b, at, p.kbytes), scale(at / BLK));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    return sum;
+}
+// the barriers of store_tile, for waves of the workgroup that have no sums
+template <class T>
+__device__ __forceinline__ void stand_by(const char* smem)
+{
+    __syncthreads();
+    __syncthreads();
+    const Doubts& d = *reinterpret_cast<const Doubts*>(smem + T::BIAS - sizeof(Doubts));
+    if (d.count > 0 && d.count <= Doubts::MAX) __syncthreads();
+}
+
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
 // sixteen rows at a time round in its own corner of LDS (a lane holds four columns of a row, a store takes neighbouring lanes along a row).  Rows of y that
 // do not start at multiples of four values are stored value by value.
@@ -274,7 +336,12 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
     const int r = lane & 15, q = lane >> 4, wm = (wave / T::WN) * T::MT * 16, wn = (wave % T::WN) * T::NT * 16;
     float* const most = reinterpret_cast<float*>(smem);                       // [wave column][row]
     char* const turn = smem + (OUT == OUT_E4M3 ? T::WN * T::BM * 4 : 0) + wave * 16 * PITCH;
-    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH <= T::BIAS, "LDS");
+    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH + sizeof(Doubts) <= T::BIAS && T::BM * (T::BN / BLK) <= 512 && T::BIAS % 16 == 0, "LDS");
+    Doubts& doubts = *reinterpret_cast<Doubts*>(smem + T::BIAS - sizeof(Doubts));
+    if constexpr (OUT == OUT_E4M3) {
+        for (int i = wave * 64 + lane; i < T::BM * (T::BN / BLK); i += T::WAVES * 64) doubts.exact[i] = 0;
+        if (wave == 0 && lane == 0) doubts.count = 0;
+    }
     f32x4 bias[T::NT];
 #pragma unroll
     for (int u = 0; u < T::NT; ++u) bias[u] = p.bias ? *reinterpret_cast<const f32x4*>(smem + T::BIAS + (wn + u * 16 + q * 4) * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -300,14 +367,43 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
     }
     if constexpr (OUT == OUT_E4M3) {
         __syncthreads();
-        const int cb = (n0 + wn) / BLK;
+        const int cb = (n0 + wn) / BLK, block = wn / BLK * T::BM;             // (of the result; of the tile)
 #pragma unroll
         for (int i = 0; i < T::MT; ++i) {
-            const int j = first + wm + i * 16 + r;
-            float t = 0.f;
+            const int lr = wm + i * 16 + r, j = first + lr;
+            top[i] = 0.f;
 #pragma unroll
-            for (int u = 0; u < PER; ++u) t = fmaxf(t, most[((wave % T::WN) / PER * PER + u) * T::BM + wm + i * 16 + r]);
-            const int e = block_exponent(t);
+            for (int u = 0; u < PER; ++u) top[i] = fmaxf(top[i], most[((wave % T::WN) / PER * PER + u) * T::BM + lr]);
+            if (in_doubt(top[i]) && source_row(p, j, end) >= 0) {
+                int c = -1;
+#pragma unroll
+                for (int u = 0; u < T::NT; ++u)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) c = n0 + wn + u * 16 + q * 4 + v < p.n && fabsf(acc[i][u][v]) == top[i] ? wn + u * 16 + q * 4 + v : c;
+                if (c >= 0) {
+                    const int at = atomicAdd(&doubts.count, 1);
+                    if (at < Doubts::MAX) doubts.where[at] = lr << 16 | c;
+                }
+            }
+        }
+        __syncthreads();
+        const int count = __builtin_amdgcn_readfirstlane(doubts.count);
+        const bool again = count > 0 && count <= Doubts::MAX;
+        if (again) {
+#pragma unroll 1
+            for (int u = wave; u < count; u += T::WAVES) {
+                const int lr = __builtin_amdgcn_readfirstlane(doubts.where[u]) >> 16, c = __builtin_amdgcn_readfirstlane(doubts.where[u]) & 0xffff;
+                float y = sum_again<IN>(p, source_row(p, first + lr, end), g, n0 + c, lane) + (p.bias ? *reinterpret_cast<const float*>(smem + T::BIAS + c * 4) : 0.f);
+                if (p.relu) y = y < 0.f ? 0.f : y;
+                if (lane == 0) atomicMax(&doubts.exact[c / BLK * T::BM + lr], __float_as_int(finite_abs(y)));
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < T::MT; ++i) {
+            const int lr = wm + i * 16 + r, j = first + lr;
+            if (again && in_doubt(top[i]) && source_row(p, j, end) >= 0) top[i] = __int_as_float(doubts.exact[block + lr]);
+            const int e = block_exponent(top[i]);
             const float inv = two_to(-e);
 #pragma unroll
             for (int u = 0; u < T::NT; ++u) acc[i][u] *= inv;
@@ -381,7 +477,7 @@ __device__ __forceinline__ bool gather_groups(f32x4 (&acc)[T::MT][T::NT], char* 
         }
         __syncthreads();
         if (kg == 1) {
-            if (OUT == OUT_E4M3) __syncthreads();                             // (store_tile's)
+            if (OUT == OUT_E4M3) stand_by<T>(smem);
             return false;
         }
     }

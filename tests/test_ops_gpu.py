@@ -195,6 +195,29 @@ def test_matmul_fp8(ops, m, n, k, scale, out):
             check(y, want, err, out, (m, n, k, relu))
 
 
+@pytest.mark.parametrize("scale", [E8, torch.float32])
+@pytest.mark.parametrize("m, n, k", [(3, 40, 128), (40, 300, 131), (600, 256, 144), (3000, 1001, 131), (1030, 2048, 256), (2000, 2048, 128), (4096, 2048, 128), (5000, 2048, 144), (8192, 2048, 256)])
+def test_scales_of_e4m3_results_next_to_a_border(ops, m, n, k, scale):
+    """A block's largest value on 448 * 2^8, and 4 to either side of it (2^-15 of it, which the 8-bit matrix instruction drops next to it): the smallest
+    exponent with max <= 448 * 2^e is 8, 8 and 9.  Every fourth row, in one block of every two."""
+    a, b = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    rows = torch.arange(m, device="cuda")
+    a[:, 0] = torch.where(rows % 4 == 0, 256.0, 1.0)
+    a[:, 1] = torch.where(rows % 4 == 0, (rows // 4 % 3 - 1) * 2.0, 0.0)
+    b[5::256, 0], b[5::256, 1], b[:, 2] = 448.0, 2.0, 1.0
+    a[:, 2] = 1.0
+    a, b = a.to(F8), b.to(F8)
+    sa, sb = torch.ones(-(-k // 128), m, device="cuda"), torch.ones(-(-n // 128), -(-k // 128), device="cuda")
+    sa, sb = (v if scale == torch.float32 else torch.full(v.shape, 127, dtype=torch.uint8, device="cuda").view(E8) for v in (sa, sb))
+    for bias in (None, torch.zeros(n, device="cuda")):
+        q, s = ops.matmul_fp8(a, sa, b, sb, bias=bias, out_dtype=F8)
+        y = a.double() @ b.double().t()
+        for t in range(-(-n // 128)):
+            e = torch.from_numpy(block_exponents(y[:, t * 128:(t + 1) * 128].abs().amax(1).cpu().numpy())).cuda()
+            assert torch.equal(number(s)[t], torch.exp2(e.double())), (t, m, n, k)
+            assert (q[:, t * 128:(t + 1) * 128].double() * number(s)[t][:, None] - y[:, t * 128:(t + 1) * 128]).abs().le(2.0 ** -4 * y[:, t * 128:(t + 1) * 128].abs() + 8).all()
+
+
 @pytest.mark.parametrize("m, n, k", [(2000, 2040, 400), (1571, 2048, 272), (4000, 2048, 656), (5000, 2040, 528), (8100, 2048, 16), (8100, 2000, 240), (8100, 2048, 1040), (3000, 1001, 419), (5000, 300, 63)])
 @pytest.mark.parametrize("form", ["bf16", E8, torch.float32])
 def test_products_whose_k_ends_inside_a_step(ops, m, n, k, form):
