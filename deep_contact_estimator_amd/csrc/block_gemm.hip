@@ -266,11 +266,12 @@ __device__ __forceinline__ void bring_bias(const ProductArgs& p, const char* sme
 
 // ---- the scale of e4m3 results.  Its exponent hangs on which side of 448 * 2^e a block's largest value lies, and the sums of the 8-bit matrix instruction are
 // good to 2^-16 of them, not to fp32: of 65536 blocks one or two would come out on the other side.  So where a largest value is within 2^-11 of such a
-// border (one block in 600) that value is summed once more, in fp32, by one wave: 3 us where a tile has such a block (2048 rows of 2048 x 4736 30.5 ->
-// 33.8 us, 4096 43.9, 32768 257 -> 271).
+// border (one block in 600) that value is summed once more, in fp32, K dealt out to all waves: 2.5 us where a tile has such
+// a block (1024 rows of 2048 x 4736 20.9 -> 23.2 us, 4096 43.5 -> 46.5, 32768 260 -> 269).
 struct Doubts {                                                               // in LDS
     static constexpr int MAX = 256;                                           // more in one tile (all values alike): it keeps its sums
     int count, where[MAX];                                                    // row << 16 | column in the tile
+    float parts[MAX][8];                                                      // the waves' sums
     int exact[512];                                                           // a block's largest value, summed again
 };
 __device__ __forceinline__ bool in_doubt(float most)
@@ -279,13 +280,17 @@ __device__ __forceinline__ bool in_doubt(float most)
     return m > -7168 && m < 7168;
 }
 template <int IN>
-__device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, int g, int c, int lane)
+__device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, int g, int c, int first, int step)          // sixteen bytes at `first`, and every `step` from there
 {
     const char* const a = p.a + src * p.a_row;
     const char* const b = p.b + g * p.b_group + (long long)c * p.b_row;
     const long long sb0 = g * p.sb_group + (long long)(c / BLK) * p.sb_row;
     float sum = 0.f;
-    auto add = [&](i32x4 x, i32x4 w, float s) {
+#pragma unroll 1
+    for (int at = first; at < p.kbytes; at += step) {
+        const bool whole = at + 16 <= p.kbytes;
+        const i32x4 x = whole ? load16(a + at) : load16_tail(a, at, p.kbytes), w = whole ? load16(b + at) : load16_tail(b, at, p.kbytes);
+        const int t = at / BLK;
         float part = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -294,24 +299,9 @@ __device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, 
             part = fmaf(__builtin_amdgcn_cvt_f32_fp8(x[i], 2), __builtin_amdgcn_cvt_f32_fp8(w[i], 2), part);
             part = fmaf(__builtin_amdgcn_cvt_f32_fp8(x[i], 3), __builtin_amdgcn_cvt_f32_fp8(w[i], 3), part);
         }
-        sum = fmaf(part, s, sum);
-    };
-    auto scale = [&](int t) {
-        if constexpr (IN == IN_F8_F32) return static_cast<const float*>(p.sa)[t * p.sa_block + src] * static_cast<const float*>(p.sb)[sb0 + t];
-        else return ldexpf(1.f, (int)static_cast<const unsigned char*>(p.sa)[t * p.sa_block + src] + (int)static_cast<const unsigned char*>(p.sb)[sb0 + t] - 254);
-    };
-    int at = lane * 16;
-#pragma unroll 1
-    for (; at + 3 * 1024 + 16 <= p.kbytes; at += 4 * 1024) {                  // (a wave's latency is what this costs: four steps' loads at once)
-        i32x4 x[4], w[4];
-        float s[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) { x[u] = load16(a + at + u * 1024); w[u] = load16(b + at + u * 1024); s[u] = scale((at + u * 1024) / BLK); }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add(x[u], w[u], s[u]);
+        if constexpr (IN == IN_F8_F32) sum = fmaf(part, static_cast<const float*>(p.sa)[t * p.sa_block + src] * static_cast<const float*>(p.sb)[sb0 + t], sum);
+        else sum += ldexpf(part, (int)static_cast<const unsigned char*>(p.sa)[t * p.sa_block + src] + (int)static_cast<const unsigned char*>(p.sb)[sb0 + t] - 254);
     }
-#pragma unroll 1
-    for (; at < p.kbytes; at += 1024) add(load16_tail(a, at, p.kbytes), load16_tail(b, at, p.kbytes), scale(at / BLK));
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
     return sum;
@@ -323,7 +313,7 @@ __device__ __forceinline__ void stand_by(const char* smem)
     __syncthreads();
     __syncthreads();
     const Doubts& d = *reinterpret_cast<const Doubts*>(smem + T::BIAS - sizeof(Doubts));
-    if (d.count > 0 && d.count <= Doubts::MAX) __syncthreads();
+    if (d.count > 0 && d.count <= Doubts::MAX) { __syncthreads(); __syncthreads(); }
 }
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
@@ -391,11 +381,20 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
         const bool again = count > 0 && count <= Doubts::MAX;
         if (again) {
 #pragma unroll 1
-            for (int u = wave; u < count; u += T::WAVES) {
-                const int lr = __builtin_amdgcn_readfirstlane(doubts.where[u]) >> 16, c = __builtin_amdgcn_readfirstlane(doubts.where[u]) & 0xffff;
-                float y = sum_again<IN>(p, source_row(p, first + lr, end), g, n0 + c, lane) + (p.bias ? *reinterpret_cast<const float*>(smem + T::BIAS + c * 4) : 0.f);
+            for (int u = 0; u < count; ++u) {
+                const int at = __builtin_amdgcn_readfirstlane(doubts.where[u]), lr = at >> 16, c = at & 0xffff;
+                const float sum = sum_again<IN>(p, source_row(p, first + lr, end), g, n0 + c, (wave * 64 + lane) * 16, T::WAVES * 1024);
+                if (lane == 0) doubts.parts[u][wave] = sum;
+            }
+            __syncthreads();
+            for (int u = wave * 64 + lane; u < count; u += T::WAVES * 64) {
+                const int lr = doubts.where[u] >> 16, c = doubts.where[u] & 0xffff;
+                float y = 0.f;
+#pragma unroll
+                for (int w = 0; w < T::WAVES; ++w) y += doubts.parts[u][w];
+                if (p.bias) y += *reinterpret_cast<const float*>(smem + T::BIAS + c * 4);
                 if (p.relu) y = y < 0.f ? 0.f : y;
-                if (lane == 0) atomicMax(&doubts.exact[c / BLK * T::BM + lr], __float_as_int(finite_abs(y)));
+                atomicMax(&doubts.exact[c / BLK * T::BM + lr], __float_as_int(finite_abs(y)));
             }
             __syncthreads();
         }
