@@ -265,19 +265,18 @@ __device__ __forceinline__ void bring_bias(const ProductArgs& p, const char* sme
 }
 
 // ---- the scale of e4m3 results.  Its exponent hangs on which side of 448 * 2^e a block's largest value lies, and the sums of the 8-bit matrix instruction are
-// good to 2^-16 of them, not to fp32: of 65536 blocks one or two would come out on the other side.  So where a largest value is within 2^-11 of such a
-// border (one block in 600) that value is summed once more, in fp32, K dealt out to all waves: 2.5 us where a tile has such
-// a block (1024 rows of 2048 x 4736 20.9 -> 23.2 us, 4096 43.5 -> 46.5, 32768 260 -> 269).
-struct Doubts {                                                               // in LDS
-    static constexpr int MAX = 256;                                           // more in one tile (all values alike): it keeps its sums
-    int count, where[MAX];                                                    // row << 16 | column in the tile
-    float parts[MAX][8];                                                      // the waves' sums
-    int exact[512];                                                           // a block's largest value, summed again
+// good to 2^-16 of them (the root of their mean square), not to fp32: of 65536 blocks one or two would come out on the other side.  So where a largest value
+// is within 2^-12 of such a border (one block in 1200) it is summed once more, in fp32, K dealt out to all waves: 1 .. 2 us a
+// tile (1024 rows of 2048 x 4736 22.9 us, to bf16 20.5; 4096 44.9 and 44.6; 32768 261 and 260).
+struct Doubts {                                                               // in LDS, by block of the tile: column block * BM + row
+    static constexpr int NONE = 0x7fffffff;
+    int any, pick[512];                                                       // the (first) column of the largest value in question
+    float parts[512][8], exact[512];                                          // the waves' sums; their sum
 };
 __device__ __forceinline__ bool in_doubt(float most)
 {
     const int m = (int)(__float_as_uint(most) & 0x7fffffu) - 0x600000;        // (448 = 1.75 * 2^8)
-    return m > -7168 && m < 7168;
+    return m > -3584 && m < 3584;                                             // (2^-12 of 0xe00000, the border with its leading bit)
 }
 template <int IN>
 __device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, int g, int c, int first, int step)          // sixteen bytes at `first`, and every `step` from there
@@ -313,7 +312,7 @@ __device__ __forceinline__ void stand_by(const char* smem)
     __syncthreads();
     __syncthreads();
     const Doubts& d = *reinterpret_cast<const Doubts*>(smem + T::BIAS - sizeof(Doubts));
-    if (d.count > 0 && d.count <= Doubts::MAX) { __syncthreads(); __syncthreads(); }
+    if (d.any) { __syncthreads(); __syncthreads(); }
 }
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
@@ -329,8 +328,8 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
     static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH + sizeof(Doubts) <= T::BIAS && T::BM * (T::BN / BLK) <= 512 && T::BIAS % 16 == 0, "LDS");
     Doubts& doubts = *reinterpret_cast<Doubts*>(smem + T::BIAS - sizeof(Doubts));
     if constexpr (OUT == OUT_E4M3) {
-        for (int i = wave * 64 + lane; i < T::BM * (T::BN / BLK); i += T::WAVES * 64) doubts.exact[i] = 0;
-        if (wave == 0 && lane == 0) doubts.count = 0;
+        for (int i = wave * 64 + lane; i < T::BM * (T::BN / BLK); i += T::WAVES * 64) doubts.pick[i] = Doubts::NONE;
+        if (wave == 0 && lane == 0) doubts.any = 0;
     }
     f32x4 bias[T::NT];
 #pragma unroll
@@ -365,43 +364,44 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
 #pragma unroll
             for (int u = 0; u < PER; ++u) top[i] = fmaxf(top[i], most[((wave % T::WN) / PER * PER + u) * T::BM + lr]);
             if (in_doubt(top[i]) && source_row(p, j, end) >= 0) {
-                int c = -1;
+                int c = Doubts::NONE;
 #pragma unroll
-                for (int u = 0; u < T::NT; ++u)
+                for (int u = T::NT - 1; u >= 0; --u)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) c = n0 + wn + u * 16 + q * 4 + v < p.n && fabsf(acc[i][u][v]) == top[i] ? wn + u * 16 + q * 4 + v : c;
-                if (c >= 0) {
-                    const int at = atomicAdd(&doubts.count, 1);
-                    if (at < Doubts::MAX) doubts.where[at] = lr << 16 | c;
-                }
+                    for (int v = 3; v >= 0; --v) c = n0 + wn + u * 16 + q * 4 + v < p.n && fabsf(acc[i][u][v]) == top[i] ? wn + u * 16 + q * 4 + v : c;
+                if (c != Doubts::NONE) { atomicMin(&doubts.pick[block + lr], c); doubts.any = 1; }
             }
         }
         __syncthreads();
-        const int count = __builtin_amdgcn_readfirstlane(doubts.count);
-        const bool again = count > 0 && count <= Doubts::MAX;
+        const bool again = __builtin_amdgcn_readfirstlane(doubts.any) != 0;
         if (again) {
+            constexpr int BLOCKS = T::BM * (T::BN / BLK);
 #pragma unroll 1
-            for (int u = 0; u < count; ++u) {
-                const int at = __builtin_amdgcn_readfirstlane(doubts.where[u]), lr = at >> 16, c = at & 0xffff;
-                const float sum = sum_again<IN>(p, source_row(p, first + lr, end), g, n0 + c, (wave * 64 + lane) * 16, T::WAVES * 1024);
-                if (lane == 0) doubts.parts[u][wave] = sum;
+            for (int u0 = 0; u0 < BLOCKS; u0 += 64) {
+                const int pick = u0 + lane < BLOCKS ? doubts.pick[u0 + lane] : Doubts::NONE;
+                for (unsigned long long left = __ballot(pick != Doubts::NONE); left; left &= left - 1) {
+                    const int b = __builtin_ctzll(left), u = u0 + b, c = __builtin_amdgcn_readlane(pick, b);
+                    const float sum = sum_again<IN>(p, source_row(p, first + u % T::BM, end), g, n0 + c, (wave * 64 + lane) * 16, T::WAVES * 1024);
+                    if (lane == 0) doubts.parts[u][wave] = sum;
+                }
             }
             __syncthreads();
-            for (int u = wave * 64 + lane; u < count; u += T::WAVES * 64) {
-                const int lr = doubts.where[u] >> 16, c = doubts.where[u] & 0xffff;
+            for (int u = wave * 64 + lane; u < BLOCKS; u += T::WAVES * 64) {
+                const int c = doubts.pick[u];
+                if (c == Doubts::NONE) continue;
                 float y = 0.f;
 #pragma unroll
                 for (int w = 0; w < T::WAVES; ++w) y += doubts.parts[u][w];
                 if (p.bias) y += *reinterpret_cast<const float*>(smem + T::BIAS + c * 4);
                 if (p.relu) y = y < 0.f ? 0.f : y;
-                atomicMax(&doubts.exact[c / BLK * T::BM + lr], __float_as_int(finite_abs(y)));
+                doubts.exact[u] = finite_abs(y);
             }
             __syncthreads();
         }
 #pragma unroll
         for (int i = 0; i < T::MT; ++i) {
             const int lr = wm + i * 16 + r, j = first + lr;
-            if (again && in_doubt(top[i]) && source_row(p, j, end) >= 0) top[i] = __int_as_float(doubts.exact[block + lr]);
+            if (again && in_doubt(top[i]) && source_row(p, j, end) >= 0) top[i] = doubts.exact[block + lr];
             const int e = block_exponent(top[i]);
             const float inv = two_to(-e);
 #pragma unroll

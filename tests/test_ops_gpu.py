@@ -218,6 +218,19 @@ def test_scales_of_e4m3_results_next_to_a_border(ops, m, n, k, scale):
             assert (q[:, t * 128:(t + 1) * 128].double() * number(s)[t][:, None] - y[:, t * 128:(t + 1) * 128]).abs().le(2.0 ** -4 * y[:, t * 128:(t + 1) * 128].abs() + 8).all()
 
 
+@pytest.mark.parametrize("m, n, k", [(70, 130, 128), (1030, 300, 131), (8192, 2048, 144)])
+def test_scales_where_every_value_is_next_to_a_border(ops, m, n, k):
+    a, b = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    a[:, 0], a[:, 1], b[:, 0], b[:, 1] = 256.0, (torch.arange(m, device="cuda") % 3 - 1) * 2.0, 448.0, 2.0
+    sa, sb = (torch.full(shape, 127, dtype=torch.uint8, device="cuda").view(E8) for shape in ((-(-k // 128), m), (-(-n // 128), -(-k // 128))))
+    q, s = ops.matmul_fp8(a.to(F8), sa, b.to(F8), sb, out_dtype=F8)
+    e = 8 + (a[:, 1] > 0).double()
+    assert torch.equal(number(s), torch.exp2(e).expand(-(-n // 128), m))
+    assert torch.equal(q.double(), torch.where(a[:, 1:2] > 0, 224.0, 448.0).double().expand(m, n))
+    again = ops.matmul_fp8(a.to(F8), sa, b.to(F8), sb, out_dtype=F8)
+    assert torch.equal(again[0].view(torch.uint8), q.view(torch.uint8)) and torch.equal(again[1].view(torch.uint8), s.view(torch.uint8))
+
+
 @pytest.mark.parametrize("m, n, k", [(2000, 2040, 400), (1571, 2048, 272), (4000, 2048, 656), (5000, 2040, 528), (8100, 2048, 16), (8100, 2000, 240), (8100, 2048, 1040), (3000, 1001, 419), (5000, 300, 63)])
 @pytest.mark.parametrize("form", ["bf16", E8, torch.float32])
 def test_products_whose_k_ends_inside_a_step(ops, m, n, k, form):
