@@ -26,7 +26,9 @@ HEAD_KEYS = [k for k, _ in STATE_DICT_SHAPES if k.startswith("fc.")]
 
 class contact_bank:
     """contact_cnn with a bank of FC heads.  precision: "bf16_fc" -- bf16 features, weights and activations, fp32 sums; "fp8_fc" -- fc.0 and
-    fc.3 in e4m3 with a power of two for every 128 values (dce.h DCE_FP8_FC), the rest bf16.  max_batch, tune: contact_cnn's."""
+    fc.3 in e4m3 with a power of two for every 128 values (dce.h DCE_FP8_FC), the rest bf16.  max_batch, tune: contact_cnn's.
+    Calls on CUDA tensors run on torch's current stream and may be captured once one has run; the conv stack's context serves one stream at a
+    time, replayed graphs included (as contact_cnn's)."""
 
     def __init__(self, device=None, max_batch: int = 32768, precision: str = "bf16_fc", tune=None):
         if precision not in ("bf16_fc", "fp8_fc"):

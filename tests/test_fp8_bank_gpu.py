@@ -265,3 +265,33 @@ def test_bank_of_one_head_is_the_model():
     assert ((got - want).abs() <= err).all()
     assert ((m.infer_sequence(seq)["logits"].double() - want).abs() <= err).all()
     m.close()
+
+
+@pytest.mark.parametrize("precision", ["bf16_fc", "fp8_fc"])
+def test_bank_on_another_stream_and_in_a_graph(precision):
+    """windows and heads replaced in place, eager calls in between; more windows than max_batch, heads outside the bank"""
+    sd = synth.make_state_dict(1, "uniform")
+    b = contact_bank(device=0, precision=precision, max_batch=512).load_state_dict(sd, [synth.make_state_dict(i + 1, "uniform") for i in range(3)])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, head = torch.randn(700, 150, 54, generator=g, device="cuda"), torch.randint(-1, 4, (700,), generator=g, device="cuda", dtype=torch.int32)
+
+    def same(got, want):
+        return all(torch.equal(torch.nan_to_num(got[k].float()), torch.nan_to_num(want[k].float())) for k in want)
+    want = b.predict(x, head)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = b.predict(x, head)
+    side.synchronize()
+    assert same(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b.predict(x, head)
+    for _ in range(3):
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        head.copy_(torch.randint(-1, 4, (700,), generator=g, device="cuda", dtype=torch.int32))
+        want = b.predict(x, head)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, want)
+    b._conv.close()
