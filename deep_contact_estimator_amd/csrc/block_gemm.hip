@@ -25,7 +25,9 @@ struct Place { int g, first, end, tn; };      // a tile: its group, its first ro
 
 // The tile of this workgroup.  Row tiles are counted group by group (offsets are held inside [0, m] whatever they say) and only here: the host knows no
 // more than a bound.  Workgroups go round the eight XCDs, so workgroup 8 i + x takes the i-th tile of the x-th eighth of those that there are: neighbours
-// share an L2: bands of eight column tiles, columns first (32 CUs: 4 x 8 tiles, 12 panels a step from beyond the L2 and 52 out of it).  64 groups a step, tiles counted by a scan over the lanes; every wave does it for itself.
+// share an L2.  They go in bands of eight column tiles, columns first: the 32 CUs of an XCD work on 4 x 8 tiles, and of the 64 panels that these take a
+// step 12 come from beyond the L2 (without bands, 8192^3: 33; 434 us, with them 410).  64 groups a step, tiles counted by a scan over the lanes; every wave
+// does it for itself.
 __device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, Place& at)
 {
     const int lane = threadIdx.x & 63;
