@@ -266,29 +266,45 @@ __device__ __forceinline__ void bring_bias(const ProductArgs& p, const char* sme
     dma4s(reinterpret_cast<const char*>(p.bias + g * p.bias_group), (unsigned)(c < p.n ? c : p.n - 1) * 4, lds_addr(smem) + T::BIAS + wave * 256);
 }
 
-// ---- the scale of e4m3 results.  Its exponent hangs on which side of 448 * 2^e a block's largest value lies, and the sums of the 8-bit matrix instruction are
-// good to 2^-16 of them (the root of their mean square), not to fp32: of 65536 blocks one or two would come out on the other side.  So where a largest value
-// is within 2^-12 of such a border (one block in 1200) it is summed once more, in fp32, K dealt out to all waves: 1 .. 2 us a
-// tile (1024 rows of 2048 x 4736 22.9 us, to bf16 20.5; 4096 44.9 and 44.6; 32768 261 and 260).
-struct Doubts {                                                               // in LDS, by block of the tile: column block * BM + row
-    static constexpr int NONE = 0x7fffffff;
-    int any, pick[512];                                                       // the (first) column of the largest value in question
-    float parts[512][8], exact[512];                                          // the waves' sums; their sum
+// ---- the scale of e4m3 results.  Its exponent hangs on which side of 448 * 2^e a block's largest value lies, and the 8-bit matrix instruction's sums may be
+// on the other side: each product loses less than 2^-13 of the largest of its group of eight, towards zero, so that a sum of products of one sign comes
+// out up to 7 * 2^-13 of itself too small (and good to fp32 otherwise).  So where a largest value lies within 2^-10 below such a border or 2^-12 above
+// it (one block in 570), every value there is summed once more in fp32, and the block lies above the border if one of them does.  The values that are
+// stored stay the first sums, which both scales hold.  Operands that cancel can be off by more (7 * 2^-13 of the sum of magnitudes), and the scale with them.
+//
+// One or two values of a row (and of a wave's columns): each by itself, K dealt out to the waves' lanes.  More: 16 x 16 at a time through the 16-bit matrix
+// instructions.  That reads 32 rows of K where a value needs two: with K 4736 it takes 7 us where one value takes 1.3.  What it costs (results in e4m3, with
+// no value ever in question, and as it is; bf16): 1024 rows of 2048 x 4736 20.3, 22.6 and 19.0 us; 4096 39.3, 42.6 and 38.0; 32768 263, 276 and 257.  Where every
+// value of 4096 rows lies on a border, 730.
+constexpr int FEW = 2, AT_ONCE = 64, MANY = 1 << 30;
+template <class T> struct Doubts {                                            // in LDS
+    unsigned blocks[8];                                                       // a bit for every 16 x 16 values of the tile with rows of many in question
+    int found;                                                                // single ones; MANY: there are such blocks
+    int list[FEW * T::BM * T::WN];                                            // row << 8 | column of the tile
+    int above[T::BM * (T::BN / BLK)];                                         // by column block * BM + row: one of them lies above the border
+    union {
+        float rows[T::WAVES][16][T::NT * 16 + 4];                             // a wave's values of sixteen rows, to look for them
+        f32x4 parts[T::WAVES][64];                                            // the waves' sums of 16 x 16 values, or of AT_ONCE single ones
+    };
 };
+constexpr int UNDER = 14336, OVER = 3584;                                     // 2^-10 and 2^-12 of 0xe00000, the border with its leading bit (448 = 1.75 * 2^8)
 __device__ __forceinline__ bool in_doubt(float most)
 {
-    const int m = (int)(__float_as_uint(most) & 0x7fffffu) - 0x600000;        // (448 = 1.75 * 2^8)
-    return m > -3584 && m < 3584;                                             // (2^-12 of 0xe00000, the border with its leading bit)
+    const int m = (int)(__float_as_uint(most) & 0x7fffffu) - 0x600000;
+    return m > -UNDER && m < OVER;
 }
-template <int IN>
-__device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, int g, int c, int first, int step)          // sixteen bytes at `first`, and every `step` from there
+__device__ __forceinline__ int border_of(float most) { return (int)((__float_as_uint(most) & 0x7f800000u) | 0x600000u); }      // (in bits)
+
+// one value: what one wave of WAVES sums of it
+template <int IN, int WAVES>
+__device__ __forceinline__ float sum_one(const ProductArgs& p, int g, long long src, int c, int wave, int lane)
 {
     const char* const a = p.a + src * p.a_row;
     const char* const b = p.b + g * p.b_group + (long long)c * p.b_row;
     const long long sb0 = g * p.sb_group + (long long)(c / BLK) * p.sb_row;
     float sum = 0.f;
 #pragma unroll 1
-    for (int at = first; at < p.kbytes; at += step) {
+    for (int at = (wave * 64 + lane) * 16; at < p.kbytes; at += WAVES * 1024) {
         const bool whole = at + 16 <= p.kbytes;
         const i32x4 x = whole ? load16(a + at) : load16_tail(a, at, p.kbytes), w = whole ? load16(b + at) : load16_tail(b, at, p.kbytes);
         const int t = at / BLK;
@@ -307,14 +323,70 @@ __device__ __forceinline__ float sum_again(const ProductArgs& p, long long src, 
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
     return sum;
 }
+// 16 x 16 values: one wave's steps (of WAVES) of their sums, as the few-rows kernel makes them: row lane & 15 of either operand
+template <int IN, int WAVES, int U>
+__device__ __forceinline__ f32x4 sum_many(const ProductArgs& p, int g, int row, int end, int col, int wave, int lane)
+{
+    const int r = lane & 15, q = lane >> 4, c = col + r, whole = p.kbytes / KROW;
+    const long long s0 = source_row(p, row + r, end), src = s0 < 0 ? 0 : s0, sb0 = g * p.sb_group + (long long)(col / BLK) * p.sb_row;
+    const char* const x_row = p.a + src * p.a_row + q * 16;
+    const char* const w_row = p.b + g * p.b_group + (long long)(c < p.n ? c : p.n - 1) * p.b_row + q * 16;
+    f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+    unsigned bad = 0;
+    auto scale_at = [&](int s, unsigned& sw, unsigned& sx) {
+        if constexpr (IN == IN_F8_F32) { sw = static_cast<const unsigned*>(p.sb)[sb0 + s]; sx = static_cast<const unsigned*>(p.sa)[s * p.sa_block + src]; }
+        else { sw = static_cast<const unsigned char*>(p.sb)[sb0 + s]; sx = static_cast<const unsigned char*>(p.sa)[s * p.sa_block + src]; }
+    };
+    auto add = [&](i32x4 w0, i32x4 w1, i32x4 x0, i32x4 x1, unsigned sw, unsigned sx) {
+        Frag<IN, true> wf[1], xf;
+        Scale<IN, true> sc;
+        wf[0].set(w0, w1, sw);
+        xf.set(x0, x1, sx);
+        sc.set(sw, sx, bad);
+        mac_row<IN, true, 1>(acc, wf, xf, sc);
+    };
+#pragma unroll 1
+    for (int s = wave; s < whole; s += WAVES * U) {
+        i32x4 w[U][2], x[U][2];
+        unsigned sw[U], sx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = s + u * WAVES;
+            if (t >= whole) continue;
+            w[u][0] = load16(w_row + t * KROW); w[u][1] = load16(w_row + t * KROW + 64);
+            x[u][0] = load16(x_row + t * KROW); x[u][1] = load16(x_row + t * KROW + 64);
+            scale_at(t, sw[u], sx[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) if (s + u * WAVES < whole) add(w[u][0], w[u][1], x[u][0], x[u][1], sw[u], sx[u]);
+    }
+    if (p.kbytes % KROW && whole % WAVES == wave) {
+        const int at = whole * KROW + q * 16;
+        unsigned sw, sx;
+        scale_at(whole, sw, sx);
+        add(load16_tail(w_row - q * 16, at, p.kbytes), load16_tail(w_row - q * 16, at + 64, p.kbytes), load16_tail(x_row - q * 16, at, p.kbytes), load16_tail(x_row - q * 16, at + 64, p.kbytes), sw, sx);
+    }
+    return acc[0];
+}
+// f(block) for the blocks with many.  Every wave of the workgroup sees the same ones.
+template <class T, class F>
+__device__ __forceinline__ void blocks_of(const Doubts<T>& d, F f)
+{
+    const int bits = (int)d.blocks[threadIdx.x & 7];
+#pragma unroll 1
+    for (int w = 0; w < 8; ++w)
+        for (unsigned left = (unsigned)__builtin_amdgcn_readlane(bits, w); left; left &= left - 1) f(w * 32 + __builtin_ctz(left));
+}
 // the barriers of store_tile, for waves of the workgroup that have no sums
 template <class T>
 __device__ __forceinline__ void stand_by(const char* smem)
 {
     __syncthreads();
     __syncthreads();
-    const Doubts& d = *reinterpret_cast<const Doubts*>(smem + T::BIAS - sizeof(Doubts));
-    if (d.any) { __syncthreads(); __syncthreads(); }
+    const Doubts<T>& d = *reinterpret_cast<const Doubts<T>*>(smem + T::BIAS - sizeof(Doubts<T>));
+    const int found = __builtin_amdgcn_readfirstlane(d.found);
+    for (int i = found & ~MANY; i > 0; i -= AT_ONCE) { __syncthreads(); __syncthreads(); }
+    if (found & MANY) blocks_of<T>(d, [](int) { __syncthreads(); __syncthreads(); });
 }
 
 // What a tile kernel does with its sums: bias, ReLU, the scale of a row's 128 columns, and stores of whole 16-byte pieces of rows: a wave turns
@@ -327,83 +399,129 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
     const int r = lane & 15, q = lane >> 4, wm = (wave / T::WN) * T::MT * 16, wn = (wave % T::WN) * T::NT * 16;
     float* const most = reinterpret_cast<float*>(smem);                       // [wave column][row]
     char* const turn = smem + (OUT == OUT_E4M3 ? T::WN * T::BM * 4 : 0) + wave * 16 * PITCH;
-    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH + sizeof(Doubts) <= T::BIAS && T::BM * (T::BN / BLK) <= 512 && T::BIAS % 16 == 0, "LDS");
-    Doubts& doubts = *reinterpret_cast<Doubts*>(smem + T::BIAS - sizeof(Doubts));
+    using D = Doubts<T>;
+    static_assert(T::WN * T::BM * 4 + T::WAVES * 16 * PITCH + sizeof(D) <= T::BIAS && T::BM * T::BN <= 256 * 256 && T::BN <= 256 && sizeof(D) % 16 == 0 && T::BIAS % 16 == 0, "LDS");
+    D& doubts = *reinterpret_cast<D*>(smem + T::BIAS - sizeof(D));
     if constexpr (OUT == OUT_E4M3) {
-        for (int i = wave * 64 + lane; i < T::BM * (T::BN / BLK); i += T::WAVES * 64) doubts.pick[i] = Doubts::NONE;
-        if (wave == 0 && lane == 0) doubts.any = 0;
+        for (int i = wave * 64 + lane; i < T::BM * (T::BN / BLK); i += T::WAVES * 64) doubts.above[i] = 0;
+        if (wave == 0 && lane < 8) doubts.blocks[lane] = 0;
+        if (wave == 0 && lane == 8) doubts.found = 0;
     }
-    f32x4 bias[T::NT];
+    auto finish = [&](float sum, float b) { const float y = sum + b; return p.relu && y < 0.f ? 0.f : y; };      // (NaN stays)
+    auto bias_of = [&](int c) { return p.bias ? *reinterpret_cast<const f32x4*>(smem + T::BIAS + (c + q * 4) * 4) : f32x4{0.f, 0.f, 0.f, 0.f}; };
+    unsigned live = 0;                                                        // the rows of this lane that have a source, a bit for each
 #pragma unroll
-    for (int u = 0; u < T::NT; ++u) bias[u] = p.bias ? *reinterpret_cast<const f32x4*>(smem + T::BIAS + (wn + u * 16 + q * 4) * 4) : f32x4{0.f, 0.f, 0.f, 0.f};
-    float top[T::MT];
+    for (int i = 0; i < T::MT; ++i) live |= source_row(p, first + wm + i * 16 + r, end) >= 0 ? 1u << i : 0;
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i) {
-        const bool none = p.index && source_row(p, first + wm + i * 16 + r, end) < 0;
-        top[i] = 0.f;
+    for (int u = 0; u < T::NT; ++u) {
+        const f32x4 bias = bias_of(wn + u * 16);
 #pragma unroll
-        for (int u = 0; u < T::NT; ++u)
+        for (int i = 0; i < T::MT; ++i)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                float y = (none ? 0.f : acc[i][u][v]) + bias[u][v];
-                if (p.relu) y = y < 0.f ? 0.f : y;                            // (NaN stays)
-                acc[i][u][v] = y;
-                if (OUT == OUT_E4M3 && n0 + wn + u * 16 + q * 4 + v < p.n) top[i] = fmaxf(top[i], finite_abs(y));
-            }
-        if constexpr (OUT == OUT_E4M3) {
-            top[i] = fmaxf(top[i], __shfl_xor(top[i], 16));
-            top[i] = fmaxf(top[i], __shfl_xor(top[i], 32));
-            if (q == 0) most[(wave % T::WN) * T::BM + wm + i * 16 + r] = top[i];
-        }
+            for (int v = 0; v < 4; ++v) acc[i][u][v] = finish(live >> i & 1 ? acc[i][u][v] : 0.f, bias[v]);
     }
     if constexpr (OUT == OUT_E4M3) {
-        __syncthreads();
         const int cb = (n0 + wn) / BLK, block = wn / BLK * T::BM;             // (of the result; of the tile)
+        auto column = [&](int u, int v) { return n0 + wn + u * 16 + q * 4 + v; };
+        float top[T::MT];
 #pragma unroll
         for (int i = 0; i < T::MT; ++i) {
-            const int lr = wm + i * 16 + r, j = first + lr;
+            float t = 0.f;
+#pragma unroll
+            for (int u = 0; u < T::NT; ++u)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) t = column(u, v) < p.n ? fmaxf(t, finite_abs(acc[i][u][v])) : t;
+            t = fmaxf(t, __shfl_xor(t, 16));
+            t = fmaxf(t, __shfl_xor(t, 32));
+            if (q == 0) most[(wave % T::WN) * T::BM + wm + i * 16 + r] = t;
+        }
+        __syncthreads();
+        unsigned many = 0, look = 0;                                          // (a bit for each of this lane's rows; for each sixteen rows)
+#pragma unroll
+        for (int i = 0; i < T::MT; ++i) {
             top[i] = 0.f;
 #pragma unroll
-            for (int u = 0; u < PER; ++u) top[i] = fmaxf(top[i], most[((wave % T::WN) / PER * PER + u) * T::BM + lr]);
-            if (in_doubt(top[i]) && source_row(p, j, end) >= 0) {
-                int c = Doubts::NONE;
-#pragma unroll
-                for (int u = T::NT - 1; u >= 0; --u)
-#pragma unroll
-                    for (int v = 3; v >= 0; --v) c = n0 + wn + u * 16 + q * 4 + v < p.n && fabsf(acc[i][u][v]) == top[i] ? wn + u * 16 + q * 4 + v : c;
-                if (c != Doubts::NONE) { atomicMin(&doubts.pick[block + lr], c); doubts.any = 1; }
-            }
+            for (int u = 0; u < PER; ++u) top[i] = fmaxf(top[i], most[((wave % T::WN) / PER * PER + u) * T::BM + wm + i * 16 + r]);
+            if (__ballot(live >> i & 1 && in_doubt(top[i]))) look |= 1u << i;
         }
-        __syncthreads();
-        const bool again = __builtin_amdgcn_readfirstlane(doubts.any) != 0;
-        if (again) {
-            constexpr int BLOCKS = T::BM * (T::BN / BLK);
+        // (What follows runs seldom, so its instructions come from far away: unrolled, 1 KB of them for every
+        // sixteen rows, 32768 rows of 2048 x 4736 took 292 us where they take 276 now.)
 #pragma unroll 1
-            for (int u0 = 0; u0 < BLOCKS; u0 += 64) {
-                const int pick = u0 + lane < BLOCKS ? doubts.pick[u0 + lane] : Doubts::NONE;
-                for (unsigned long long left = __ballot(pick != Doubts::NONE); left; left &= left - 1) {
-                    const int b = __builtin_ctzll(left), u = u0 + b, c = __builtin_amdgcn_readlane(pick, b);
-                    const float sum = sum_again<IN>(p, source_row(p, first + u % T::BM, end), g, n0 + c, (wave * 64 + lane) * 16, T::WAVES * 1024);
-                    if (lane == 0) doubts.parts[u][wave] = sum;
+        for (; look; look &= look - 1) {
+            const int i = __builtin_ctz(look);
+            float limits = 0.f;                                               // lane r: the row's largest
+#pragma unroll
+            for (int k = 0; k < T::MT; ++k)
+                if (k == i) {
+                    limits = live >> k & 1 ? top[k] : 0.f;
+#pragma unroll
+                    for (int u = 0; u < T::NT; ++u) *reinterpret_cast<f32x4*>(&doubts.rows[wave][r][u * 16 + q * 4]) = acc[k][u];
+                }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (unsigned rows = (unsigned)__ballot(q == 0 && in_doubt(limits)); rows; rows &= rows - 1) {
+                const int row = __builtin_ctz(rows), limit = border_of(__uint_as_float((unsigned)__builtin_amdgcn_readlane(__float_as_int(limits), row))) - UNDER;
+                const int y = lane < T::NT * 16 ? __float_as_int(doubts.rows[wave][row][lane]) & 0x7fffffff : 0;
+                const bool in = y > limit && y < 0x7f800000 && n0 + wn + lane < p.n;                           // (larger ones may lie above the border)
+                const unsigned long long all = __ballot(in);
+                if (__popcll(all) <= FEW) {
+                    if (in) doubts.list[atomicAdd(&doubts.found, 1)] = (wm + i * 16 + row) << 8 | (wn + lane);
+                } else {
+                    many |= r == row ? 1u << i : 0;
+                    const int b = (wm / 16 + i) * (T::BN / 16) + wn / 16 + lane;
+                    if (lane < T::NT && (all >> lane * 16 & 0xffff)) atomicOr(&doubts.blocks[b >> 5], 1u << (b & 31));
+                    if (lane == 0) atomicOr(&doubts.found, MANY);
                 }
             }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        const int state = __builtin_amdgcn_readfirstlane(doubts.found), found = state & ~MANY;
+#pragma unroll 1
+        for (int i0 = 0; i0 < found; i0 += AT_ONCE) {
+            float* const parts = reinterpret_cast<float*>(doubts.parts);
+#pragma unroll 1
+            for (int i = i0; i < found && i < i0 + AT_ONCE; ++i) {
+                const int e = __builtin_amdgcn_readfirstlane(doubts.list[i]);
+                const float sum = sum_one<IN, T::WAVES>(p, g, source_row(p, first + (e >> 8), end), n0 + (e & 255), wave, lane);
+                if (lane == 0) parts[(i - i0) * T::WAVES + wave] = sum;
+            }
             __syncthreads();
-            for (int u = wave * 64 + lane; u < BLOCKS; u += T::WAVES * 64) {
-                const int c = doubts.pick[u];
-                if (c == Doubts::NONE) continue;
-                float y = 0.f;
+            if (wave == 0 && i0 + lane < found) {                             // (the order of the list does not matter: a value says the same from any place)
+                const int e = doubts.list[i0 + lane], lr = e >> 8, c = e & 255;
+                float y = 0.f, largest = 0.f;
 #pragma unroll
-                for (int w = 0; w < T::WAVES; ++w) y += doubts.parts[u][w];
-                if (p.bias) y += *reinterpret_cast<const float*>(smem + T::BIAS + c * 4);
-                if (p.relu) y = y < 0.f ? 0.f : y;
-                doubts.exact[u] = finite_abs(y);
+                for (int w = 0; w < T::WAVES; ++w) y += parts[lane * T::WAVES + w];
+                y = finish(y, p.bias ? *reinterpret_cast<const float*>(smem + T::BIAS + c * 4) : 0.f);
+#pragma unroll
+                for (int u = 0; u < PER; ++u) largest = fmaxf(largest, most[(c / BLK * PER + u) * T::BM + lr]);
+                if ((int)(__float_as_uint(y) & 0x7fffffffu) > border_of(largest)) doubts.above[c / BLK * T::BM + lr] = 1;
             }
             __syncthreads();
         }
+        if (state & MANY) blocks_of<T>(doubts, [&](int b) {
+            const int row = b / (T::BN / 16) * 16, col = b % (T::BN / 16) * 16;
+            doubts.parts[wave][lane] = sum_many<IN, T::WAVES, T::MT * T::NT < 32 ? 2 : 1>(p, g, first + row, end, n0 + col, wave, lane);
+            __syncthreads();
+            if (row >= wm && row < wm + T::MT * 16 && col >= wn && col < wn + T::NT * 16) {
+                f32x4 y = doubts.parts[0][lane];
+#pragma unroll
+                for (int w = 1; w < T::WAVES; ++w) y += doubts.parts[w][lane];
+                const f32x4 bias = bias_of(col);
+                int border = 0x7fffffff;                                      // (rows that are summed one by one, or not at all)
+#pragma unroll
+                for (int i = 0; i < T::MT; ++i) if (row == wm + i * 16 && many >> i & 1) border = border_of(top[i]);
+                bool over = false;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) over |= n0 + col + q * 4 + v < p.n && (int)(__float_as_uint(finish(y[v], bias[v])) & 0x7fffffffu) > border;
+                if (over) doubts.above[block + row + r] = 1;
+            }
+            __syncthreads();
+        });
 #pragma unroll
         for (int i = 0; i < T::MT; ++i) {
             const int lr = wm + i * 16 + r, j = first + lr;
-            if (again && in_doubt(top[i]) && source_row(p, j, end) >= 0) top[i] = doubts.exact[block + lr];
+            if (state && live >> i & 1 && in_doubt(top[i])) top[i] = __uint_as_float((unsigned)(border_of(top[i]) + doubts.above[block + lr]));
             const int e = block_exponent(top[i]);
             const float inv = two_to(-e);
 #pragma unroll

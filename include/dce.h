@@ -377,9 +377,11 @@ int  dce_quantize(int device_id, void* hip_stream, const dce_quantize_desc* d);
  * DEVICE, never falling (NULL: one group of all m rows); they are held inside [0, m]; rows of y that no group covers stay as they were.  Operands bf16,
  * or e4m3 where a[i, k] stands for a * a_scale[(k / 128) * ld_a_scale + i] and b[g, c, k] for b * b_scale[g * b_scale_group + (c / 128) * ld_b_scale +
  * k / 128].  fp32 scales may be any finite numbers whose products are normal fp32 numbers or zero; e8m0 scales any, but a value that is no normal fp32
- * number (448 * 2^120, 2^-9 * 2^-120) may count as infinite or as zero.  Sums are fp32 (of e4m3 operands with results in bf16 or
- * e4m3: groups of eight products keep 13 bits below their largest, 2^-16 of a result); y is rounded once to y_type; e4m3 results take dce_quantize's power
- * of two for every 128 columns of a row, y_scale[(c / 128) * ld_y_scale + j], in scale_type.  Any m, n and k (k = 0: the bias); strides in values; 16-byte
+ * number (448 * 2^120, 2^-9 * 2^-120) may count as infinite or as zero.  Sums are fp32; of e4m3 operands with results in bf16
+ * or e4m3, a product of a group of eight loses less than 2^-13 of the group's largest besides: a sum is off by up to 7 * 2^-13 of the sum of its products'
+ * magnitudes (1.5e-5 of a result on random operands, 7e-5 where all have one sign, and any part of one that cancels).  y is rounded once to y_type; e4m3
+ * results take dce_quantize's power of two for every 128 columns of a row, y_scale[(c / 128) * ld_y_scale + j], in scale_type: that of the exact sums where
+ * products and bias have one sign (values near a border are summed again in fp32), otherwise that of sums off by no more than the above.  Any m, n and k (k = 0: the bias); strides in values; 16-byte
  * aligned rows run fastest.  y overlaps neither a nor b (refused where it is found to).  The same call gives the same bits. */
 typedef struct dce_matmul_desc {
     const void* a; int64_t lda; const void* a_scale; int64_t ld_a_scale;
