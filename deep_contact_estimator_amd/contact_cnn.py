@@ -163,7 +163,7 @@ class contact_cnn:
             import torch
             if x.device.index != self._dev_index:
                 raise RuntimeError(f"input on cuda:{x.device.index}, model on cuda:{self._dev_index}")
-            x = x.contiguous()
+            x = x.resolve_neg().contiguous()
             if x.dtype != torch.float32:
                 x = x.float()
             n = x.shape[0] - (WINDOW - 1) if raw_sequence else x.shape[0]
@@ -245,7 +245,7 @@ class contact_cnn:
         ctx, lib = self._ctx, self._lib
         if _is_torch(x) and x.is_cuda:
             import torch
-            x = x.contiguous()
+            x = x.resolve_neg().contiguous()
             if x.dtype != torch.float32:
                 x = x.float()
             n = max(x.shape[0] - (WINDOW - 1) if raw_sequence else x.shape[0], 0)
@@ -407,7 +407,7 @@ class contact_cnn:
         self._finalize()
         if x.device.index != self._dev_index:
             raise RuntimeError(f"input on cuda:{x.device.index}, model on cuda:{self._dev_index}")
-        x = x.contiguous().float()
+        x = x.resolve_neg().contiguous().float()
         n = max(x.shape[0] - (WINDOW - 1) if raw_sequence else x.shape[0], 0)
         out = torch.empty((n, 4736), dtype=torch.bfloat16, device=x.device)
         self._torch_stream(x)
@@ -441,7 +441,7 @@ class contact_cnn:
             n = T - (WINDOW - 1) - first
         if _is_torch(seq) and seq.is_cuda:
             import torch
-            seq = seq.contiguous()
+            seq = seq.resolve_neg().contiguous()
             out = torch.empty((n, WINDOW, CHANNELS), dtype=torch.float32, device=seq.device)
             _lib.check(self._lib.dce_set_stream(ctx, C.c_void_p(torch.cuda.current_stream(seq.device).cuda_stream), 0), ctx)
             self._online_stream_own = False

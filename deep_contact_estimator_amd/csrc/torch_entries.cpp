@@ -41,12 +41,16 @@ std::string text(at::IntArrayRef s)
     return t + (s.size() == 1 ? ",)" : ")");
 }
 
-// a tensor argument; None: an undefined tensor
-at::Tensor tensor(PyObject* o, const char* what)
+// a tensor argument; None: an undefined tensor.  What the kernels read is a tensor's memory, so a view that stands for the negative of its memory is made
+// into what it stands for; written to, it would hold the negative of the result.
+at::Tensor tensor(PyObject* o, const char* what, bool written = false)
 {
     if (o == Py_None) return {};
     if (!THPVariable_Check(o)) refuse("%s: expected a tensor, got %s", what, Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
+    at::Tensor t = THPVariable_Unpack(o);
+    if (!t.is_neg()) return t;
+    if (written) refuse("%s: out and out_scale cannot be views that stand for the negative of their memory", what);
+    return t.resolve_neg();
 }
 
 int device_of(const at::Tensor& t, const char* what)
@@ -147,8 +151,8 @@ PyObject* matmul(PyObject* const* arg)
 {
     const char* what = PyUnicode_AsUTF8(arg[0]);
     if (!what) throw Refused{};
-    at::Tensor a = tensor(arg[1], what), as = tensor(arg[2], what), b = tensor(arg[3], what), bs = tensor(arg[4], what), bias = tensor(arg[5], what), out = tensor(arg[8], what),
-               outs = tensor(arg[9], what), offsets = tensor(arg[10], what), index = tensor(arg[11], what);
+    at::Tensor a = tensor(arg[1], what), as = tensor(arg[2], what), b = tensor(arg[3], what), bs = tensor(arg[4], what), bias = tensor(arg[5], what), out = tensor(arg[8], what, true),
+               outs = tensor(arg[9], what, true), offsets = tensor(arg[10], what), index = tensor(arg[11], what);
     const int relu = PyObject_IsTrue(arg[6]);
     const long out_type = PyLong_AsLong(arg[7]);
     if (relu < 0 || (out_type == -1 && PyErr_Occurred())) throw Refused{};

@@ -1,0 +1,46 @@
+"""GPU: tensors that are not what their memory holds, and tensors of autograd: the operators take them as torch's own do, or refuse them."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from deep_contact_estimator_amd import contact_cnn, ops, synth   # noqa: E402
+
+
+def same(a, b):
+    return all(torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8)) for x, y in zip(a, b))
+
+
+def test_views_that_stand_for_the_negative_of_their_memory():
+    """such a view and a tensor of its values give the same bits"""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(70, 256, generator=g, device="cuda")
+    neg, plain = torch._neg_view(x), -x
+    assert neg.is_neg() and torch.equal(neg, plain)
+    assert same(ops.quantize(neg), ops.quantize(plain))
+    assert same(ops.quantize(neg, rows=128), ops.quantize(plain, rows=128))
+    conj = torch.complex(x, x + 1).conj().imag                     # (how such views come about)
+    assert conj.is_neg() and same(ops.quantize(conj), ops.quantize(-(x + 1)))
+    w, offsets = torch.randn(2, 48, 256, generator=g, device="cuda").bfloat16(), torch.tensor([0, 30, 70], dtype=torch.int32, device="cuda")
+    bias = torch.randn(2, 48, generator=g, device="cuda")
+    a = x.bfloat16()
+    want = ops.matmul_grouped(-a, w, offsets, bias=-bias)
+    assert torch.equal(ops.matmul_grouped(torch._neg_view(a), w, offsets, bias=torch._neg_view(bias)), want)
+    assert torch.equal(ops.matmul_grouped(-a, torch._neg_view(-w), offsets, bias=-bias), want)
+    v = torch.randn(40, 16, generator=g, device="cuda")
+    got, want = ops.decide(torch._neg_view(v)), ops.decide(-v)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    out = torch.zeros(70, 48, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="negative of their memory"):
+        ops.matmul_grouped(a, w, offsets, out=torch._neg_view(out))
+
+
+def test_the_models_too():
+    x = torch.randn(3, 150, 54, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    for precision in ("fp32", "bf16_fc"):
+        m = contact_cnn(device=0, precision=precision, max_batch=8)
+        m.load_state_dict(synth.make_state_dict(1, "uniform")).eval()
+        assert torch.equal(m(torch._neg_view(x)), m(-x))
+        if precision == "bf16_fc":
+            assert torch.equal(m.features(torch._neg_view(x)), m.features(-x))
+        m.close()
