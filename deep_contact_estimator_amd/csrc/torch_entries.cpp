@@ -6,6 +6,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 
 #include "../../include/dce.h"
@@ -62,11 +63,12 @@ int device_of(const at::Tensor& t, const char* what)
 
 void same(int dev, const char* what, std::initializer_list<const at::Tensor*> all)
 {
-    const bool grad = at::GradMode::is_enabled();
+    const bool grad = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const at::Tensor* t : all) {
         if (!t->defined()) continue;
         if (!t->is_cuda() || t->get_device() != dev) refuse("%s: tensors on cuda:%d and on %s", what, dev, t->device().str().c_str());
         if (grad && t->requires_grad()) refuse("%s: deep_contact_estimator_amd implements the inference path only: detach the tensor, or call under torch.no_grad()", what);
+        if (forward && t->_fw_grad(0).defined()) refuse("%s: deep_contact_estimator_amd implements the inference path only: this tensor has a tangent, which the result would lose; unpack the dual tensor", what);
     }
 }
 

@@ -44,3 +44,22 @@ def test_the_models_too():
         if precision == "bf16_fc":
             assert torch.equal(m.features(torch._neg_view(x)), m.features(-x))
         m.close()
+
+
+def test_tangents_are_refused_and_not_lost():
+    """a dual tensor of forward-mode differentiation, as any operand; its primal alone is an ordinary tensor"""
+    import torch.autograd.forward_ad as fw
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, w, v = (torch.randn(*s, generator=g, device="cuda") for s in ((8, 128), (1, 16, 128), (5, 16)))
+    a, b, offsets, bias = x.bfloat16(), w.bfloat16(), torch.tensor([0, 8], dtype=torch.int32, device="cuda"), torch.zeros(1, 16, device="cuda")
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))      # noqa: E731
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad():
+                for call in (lambda: ops.quantize(dual(x)), lambda: ops.decide(dual(v)), lambda: ops.matmul_grouped(dual(a), b, offsets),
+                             lambda: ops.matmul_grouped(a, dual(b), offsets), lambda: ops.matmul_grouped(a, b, offsets, bias=dual(bias))):
+                    with pytest.raises(RuntimeError, match="tangent"):
+                        call()
+        assert same(ops.quantize(fw.unpack_dual(dual(x)).primal), ops.quantize(x))
+        with torch.inference_mode():
+            assert same(ops.quantize(x), ops.quantize(x.clone()))
