@@ -90,13 +90,17 @@ class contact_bank:
 
     def _run(self, x, head, raw_sequence: bool):
         import torch
+        if not _is_torch(head):
+            head = torch.from_numpy(np.ascontiguousarray(head))
+        if head.dtype.is_floating_point or head.dtype.is_complex:
+            raise RuntimeError(f"contact_bank: head must be whole numbers, got {head.dtype}")     # (-0.5 is no head: rounded towards zero it would be one)
         host = not (_is_torch(x) and x.is_cuda)
         if host:
             self._conv._ensure_ctx()
             at = torch.device("cuda", self._conv._dev_index)
             x = (x if _is_torch(x) else torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32))).to(at)
         feat = self._conv.features(x, raw_sequence)
-        head = (head if _is_torch(head) else torch.from_numpy(np.ascontiguousarray(head))).to(feat.device)
+        head = head.to(feat.device)
         if head.dtype not in (torch.int32, torch.int64):
             head = head.long()
         if tuple(head.shape) != (feat.shape[0],):
