@@ -32,6 +32,16 @@ bool apart(const Rows& a, const Rows& b)
     const int64_t d = a.at <= b.at ? (int64_t)((b.at - a.at) % a.stride) : (a.stride - (int64_t)((a.at - b.at) % a.stride)) % a.stride;
     return d >= a.width && d + b.width <= a.stride;
 }
+// `count` matrices of the same rows, `step` bytes apart (0: one), and one that is written: none of them in its place?
+bool apart(const Rows& r, int64_t count, int64_t step, const Rows& w)
+{
+    if (step == 0) count = 1;
+    if (r.rows < 1 || r.width < 1 || w.rows < 1 || w.width < 1 || w.end() <= r.at || r.end() + (uintptr_t)((count - 1) * step) <= w.at) return true;
+    for (int64_t g = 0; g < count; ++g) { Rows m = r; m.at += (uintptr_t)(g * step); if (!apart(m, w)) return false; }
+    return true;
+}
+// one run of n values
+Rows run(const void* p, int64_t n, int64_t size) { return Rows(p, p && n > 0 ? 1 : 0, n, n, size); }
 // rows that no address space holds (so that no offset below passes 64 bits)
 bool endless(int64_t rows, int64_t ld, int size) { return rows > 1 && ld > (1ll << 47) / size / (rows - 1); }
 
@@ -71,8 +81,15 @@ int dce_quantize(int device_id, void* hip_stream, const dce_quantize_desc* d)
     const int es = d->x_type == DCE_TYPE_F32 ? 4 : 2;
     if (off(d->x, es) || (d->scale_type == DCE_SCALE_F32 && off(d->scale, 4))) return fail(nullptr, DCE_ERR_ARG, "dce_quantize: a pointer is not aligned to its type");
     if (d->block_rows == 1 && d->ld_scale < d->rows) return fail(nullptr, DCE_ERR_ARG, "dce_quantize: ld_scale %lld is below the rows (%lld)", (long long)d->ld_scale, (long long)d->rows);
+    if (endless(d->batch, d->x_batch, 4) || endless(d->batch, d->q_batch, 4) || endless((d->k + BLK - 1) / BLK, d->block_rows == 1 ? d->ld_scale : 0, 4))
+        return fail(nullptr, DCE_ERR_ARG, "dce_quantize: a stride is out of range (x_batch %lld, q_batch %lld, ld_scale %lld)", (long long)d->x_batch, (long long)d->q_batch, (long long)d->ld_scale);
     const Rows x(d->x, d->rows, d->ldx, d->k, es), q(d->q, d->rows, d->ldq, d->k, 1);
-    if (d->batch == 1 && !apart(x, q)) return fail(nullptr, DCE_ERR_ARG, "dce_quantize: x and q overlap");
+    const int64_t kb = (d->k + BLK - 1) / BLK, ss = d->scale_type == DCE_SCALE_F32 ? 4 : 1;
+    const Rows scale = d->block_rows == 1 ? Rows(d->scale, kb, d->ld_scale, d->rows, ss) : run(d->scale, d->batch * ((d->rows + BLK - 1) / BLK) * kb, ss);
+    bool clear = apart(x, d->batch, d->x_batch * es, scale) && apart(q, d->batch, d->q_batch, scale);
+    const bool far = q.end() + (uintptr_t)((d->batch - 1) * d->q_batch) <= x.at || x.end() + (uintptr_t)((d->batch - 1) * d->x_batch * es) <= q.at;
+    for (int64_t g = 0; clear && !far && g < d->batch; ++g) { Rows w = q; w.at += (uintptr_t)(g * d->q_batch); clear = apart(x, d->batch, d->x_batch * es, w); }
+    if (!clear) return fail(nullptr, DCE_ERR_ARG, "dce_quantize: x, q and scale overlap");
     OP_DEVICE(device_id);
     QuantArgs a{};
     a.x = static_cast<const char*>(d->x); a.x_row = x.stride; a.x_batch = d->x_batch * es;
@@ -102,11 +119,13 @@ int dce_matmul(int device_id, void* hip_stream, const dce_matmul_desc* d)
     if (endless(d->a_rows, d->lda, 4) || endless(d->n, d->ldb, 4) || endless(d->m, d->ldy, 4))
         return fail(nullptr, DCE_ERR_ARG, "dce_matmul: a row stride is out of range (a %lld, b %lld, y %lld)", (long long)d->lda, (long long)d->ldb, (long long)d->ldy);
     if (d->groups > 1 && (d->b_group < 0 || d->bias_group < 0 || d->b_scale_group < 0)) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: a group stride is negative");
-    if (endless(d->groups, d->b_group, 4)) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: a group stride is out of range");
+    const int64_t kb = (d->k + BLK - 1) / BLK, nb = (d->n + BLK - 1) / BLK;
+    if (endless(kb, d->ld_a_scale, 4) || endless(nb, d->ld_b_scale, 4) || (d->out_type == DCE_TYPE_E4M3 && endless(nb, d->ld_y_scale, 4)))
+        return fail(nullptr, DCE_ERR_ARG, "dce_matmul: a scale's stride is out of range (a %lld, b %lld, y %lld)", (long long)d->ld_a_scale, (long long)d->ld_b_scale, (long long)d->ld_y_scale);
+    if (endless(d->groups, d->b_group, 4) || endless(d->groups, d->bias_group, 4) || endless(d->groups, d->b_scale_group, 4)) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: a group stride is out of range");
     if (d->m == 0 || d->n == 0) return DCE_OK;
     if (!d->y || (d->k && (!d->b || (!d->a && d->a_rows)))) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: NULL argument");
     const int es = f8 ? 1 : 2, os = d->out_type == DCE_TYPE_F32 ? 4 : d->out_type == DCE_TYPE_BF16 ? 2 : 1;
-    const int64_t kb = (d->k + BLK - 1) / BLK, nb = (d->n + BLK - 1) / BLK;
     if (f8 && d->k) {
         if (!d->a_scale && d->a_rows) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: e4m3 operands need a_scale and b_scale");
         if (!d->b_scale) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: e4m3 operands need a_scale and b_scale");
@@ -119,10 +138,16 @@ int dce_matmul(int device_id, void* hip_stream, const dce_matmul_desc* d)
     }
     if (off(d->a, es) || off(d->b, es) || off(d->y, os) || off(d->bias, 4) || off(d->offsets, 4) || off(d->index, 4)) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: a pointer is not aligned to its type");
     const Rows a(d->a, d->a_rows, d->lda, d->k, es), b(d->b, d->n, d->ldb, d->k, es), y(d->y, d->m, d->ldy, d->n, os);
-    bool clear = apart(a, y);
-    if (clear && d->k && y.at < b.end() + (d->groups - 1) * d->b_group * es && b.at < y.end())
-        for (int g = 0; clear && g < d->groups; ++g) { Rows w = b; w.at += (uintptr_t)(g * d->b_group * es); clear = apart(w, y); }
-    if (!clear) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: y overlaps an operand");
+    // workgroups run in any order: nothing that one may still read is written by another
+    const int ss = d->scale_type == DCE_SCALE_F32 ? 4 : 1;
+    const Rows sa(d->a_scale, f8 && d->a_scale ? kb : 0, d->ld_a_scale, d->a_rows, ss), sb(d->b_scale, f8 && d->b_scale ? nb : 0, d->ld_b_scale, kb, ss);
+    const Rows ys(d->y_scale, d->out_type == DCE_TYPE_E4M3 ? nb : 0, d->ld_y_scale, d->m, ss);
+    const Rows offsets = run(d->offsets, d->groups + 1, 4), index = run(d->index, d->m, 4), bias = run(d->bias, d->n, 4);
+    auto clear_of_reads = [&](const Rows& w) {
+        return (!d->k || (apart(a, w) && apart(b, d->groups, d->b_group * es, w) && apart(sa, w) && apart(sb, d->groups, d->b_scale_group * ss, w))) &&
+               apart(bias, d->groups, d->bias_group * 4, w) && apart(offsets, w) && apart(index, w);
+    };
+    if (!clear_of_reads(y) || !clear_of_reads(ys) || !apart(y, ys)) return fail(nullptr, DCE_ERR_ARG, "dce_matmul: y or y_scale overlaps an operand, a scale, the bias, offsets or index, or one the other");
     OP_DEVICE(device_id);
     ProductArgs p{};
     p.a = static_cast<const char*>(d->a); p.a_row = a.stride;
@@ -156,6 +181,12 @@ int dce_group_rows(int device_id, void* hip_stream, const void* ids, int id_byte
     if (!offsets || (n && (!ids || !order || !place))) return fail(nullptr, DCE_ERR_ARG, "dce_group_rows: NULL argument");
     if (!work && group_rows_work(n, groups)) return fail(nullptr, DCE_ERR_ARG, "dce_group_rows: %lld rows need dce_group_rows_work's workspace", (long long)n);
     if (off(ids, id_bytes) || off(offsets, 4) || off(order, 4) || off(place, 4) || off(work, 4)) return fail(nullptr, DCE_ERR_ARG, "dce_group_rows: a pointer is not aligned to its type");
+    const Rows in = run(ids, n, id_bytes), out[4] = {run(offsets, groups + 1, 4), run(order, n, 4), run(place, n, 4), run(work, group_rows_work(n, groups), 4)};
+    for (int i = 0; i < 4; ++i) {
+        bool clear = apart(in, out[i]);
+        for (int j = 0; clear && j < i; ++j) clear = apart(out[j], out[i]);
+        if (!clear) return fail(nullptr, DCE_ERR_ARG, "dce_group_rows: ids, offsets, order, place and work overlap");
+    }
     OP_DEVICE(device_id);
     HIP_TRY(nullptr, launch_group_rows(ids, id_bytes, (int)n, groups, offsets, order, place, work, (hipStream_t)hip_stream));
     return DCE_OK;
@@ -168,6 +199,14 @@ int dce_decide(int device_id, void* hip_stream, const float* logits, int64_t row
     if (n == 0) return DCE_OK;
     if (!logits && rows) return fail(nullptr, DCE_ERR_ARG, "dce_decide: NULL argument");
     if (off(logits, 4) || off(index, 4) || off(logits_out, 4) || off(pred, 4)) return fail(nullptr, DCE_ERR_ARG, "dce_decide: a pointer is not aligned to its type");
+    if (rows > (1ll << 42)) return fail(nullptr, DCE_ERR_ARG, "dce_decide: %lld rows", (long long)rows);
+    const Rows in = run(logits, rows * 16, 4), at = run(index, n, 4), out[3] = {run(logits_out, n * 16, 4), run(pred, n, 4), run(contacts, n * 4, 1)};
+    for (int i = 0; i < 3; ++i) {
+        const bool in_place = i == 0 && logits_out == logits && !index;      // (a row's lanes read it and then write it)
+        bool clear = (in_place || apart(in, out[i])) && apart(at, out[i]);
+        for (int j = 0; clear && j < i; ++j) clear = apart(out[j], out[i]);
+        if (!clear) return fail(nullptr, DCE_ERR_ARG, "dce_decide: logits, index and the results overlap");
+    }
     OP_DEVICE(device_id);
     HIP_TRY(nullptr, launch_decide(logits, n, rows, index, logits_out, pred, contacts, (hipStream_t)hip_stream));
     return DCE_OK;

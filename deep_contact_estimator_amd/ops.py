@@ -67,7 +67,8 @@ def matmul_fp8(a, a_scale, b, b_scale, bias=None, relu: bool = False, out_dtype=
     drops less than 2^-13 of the largest of eight products from each of the others: sums are off by up to 7 * 2^-13 of the sum of
     their products' magnitudes, 1.5e-5 of a result on random operands; where products cancel, more of it, and an e4m3 scale may
     follow (include/dce.h).  An operand's value that is no normal float32 number may count as infinite or as zero.  out may lie
-    beside a and b in one tensor, not on them.  Any sizes and row strides; rows that start at multiples of 16 bytes run fastest."""
+    beside a and b in one tensor; out and out_scale overlap nothing that the call reads, nor each other.  Any sizes and row strides;
+    rows that start at multiples of 16 bytes run fastest."""
     return _entries().matmul("matmul_fp8", a, a_scale, b, b_scale, bias, relu, _out("matmul_fp8", out_dtype), out, out_scale, None, None)
 
 

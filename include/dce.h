@@ -362,7 +362,7 @@ typedef enum dce_scale { DCE_SCALE_E8M0 = 0, DCE_SCALE_F32 = 1 } dce_scale;     
 /* x -> e4m3 and a power of two for every block: e = the smallest with max|x| <= 448 * 2^e, held inside [-126, 120]; q = x * 2^-e rounded once, ties to
  * even.  NaN and infinities become NaN and are left out of the maximum.  block_rows 1: activations, one matrix (batch 1), scale of row i and block t at
  * scale[t * ld_scale + i].  block_rows 128: weights, `batch` matrices, scale (batch, ceil(rows / 128), ceil(k / 128)) without gaps.  Any k; strides are
- * in values; x and q may not overlap (refused where one matrix's do). */
+ * in values; x, q and scale may not overlap (refused). */
 typedef struct dce_quantize_desc {
     const void* x;  int64_t ldx, x_batch;
     uint8_t*    q;  int64_t ldq, q_batch;
@@ -382,7 +382,8 @@ int  dce_quantize(int device_id, void* hip_stream, const dce_quantize_desc* d);
  * magnitudes (1.5e-5 of a result on random operands, 7e-5 where all have one sign, and any part of one that cancels).  y is rounded once to y_type; e4m3
  * results take dce_quantize's power of two for every 128 columns of a row, y_scale[(c / 128) * ld_y_scale + j], in scale_type: that of the exact sums where
  * products and bias have one sign (values near a border are summed again in fp32), otherwise that of sums off by no more than the above.  Any m, n and k (k = 0: the bias); strides in values; 16-byte
- * aligned rows run fastest.  y overlaps neither a nor b (refused where it is found to).  The same call gives the same bits. */
+ * aligned rows run fastest.  y and y_scale overlap nothing that the
+ * call reads, nor each other (refused where they are found to: rows of different strides that interleave are not looked into).  The same call gives the same bits. */
 typedef struct dce_matmul_desc {
     const void* a; int64_t lda; const void* a_scale; int64_t ld_a_scale;
     const void* b; int64_t ldb, b_group; const void* b_scale; int64_t ld_b_scale, b_scale_group;
@@ -396,13 +397,15 @@ int  dce_matmul(int device_id, void* hip_stream, const dce_matmul_desc* d);
 
 /* Rows in the order of their group: ids (n) int32 or int64 (id_bytes 4 | 8) -> offsets (groups + 1), order (n: the row at every place, rows of a group in
  * their own order, -1 behind the last group), place (n: the place of every row; -1 for an id outside [0, groups), which belongs to no group).  work:
- * dce_group_rows_work(n, groups) int32 of device memory (may be 0), used by this call alone until it has run. */
+ * dce_group_rows_work(n, groups) int32 of device memory (may be 0), used by this call alone until it has run.  The five overlap
+ * nowhere (refused). */
 int64_t dce_group_rows_work(int64_t n, int groups);
 int  dce_group_rows(int device_id, void* hip_stream, const void* ids, int id_bytes, int64_t n, int groups,
                     int32_t* offsets, int32_t* order, int32_t* place, int32_t* work);
 
 /* torch.max(output, 1) + decimal2binary (src/inference_one_seq.py:25-27) on (rows, 16) logits picked by index (n; NULL: rows 0 .. n - 1): logits_out
- * (n, 16), pred (n), contacts (n, 4), any may be NULL.  An index outside [0, rows): NaN logits, and so class 0. */
+ * (n, 16), pred (n), contacts (n, 4), any may be NULL.  An index outside [0, rows): NaN logits, and so class 0.  Without an index
+ * logits_out may be logits; nothing overlaps otherwise (refused). */
 int  dce_decide(int device_id, void* hip_stream, const float* logits, int64_t rows, const int32_t* index, int64_t n,
                 float* logits_out, int32_t* pred, uint8_t* contacts);
 

@@ -63,3 +63,15 @@ def test_tangents_are_refused_and_not_lost():
         assert same(ops.quantize(fw.unpack_dual(dual(x)).primal), ops.quantize(x))
         with torch.inference_mode():
             assert same(ops.quantize(x), ops.quantize(x.clone()))
+
+
+def test_results_on_the_scales_that_a_product_reads_are_refused():
+    x, w = torch.randn(256, 256, device="cuda"), torch.randn(256, 256, device="cuda")
+    (q, s), (b, bs) = ops.quantize(x), ops.quantize(w, rows=128)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.matmul_fp8(q, s, b, bs, out_dtype=torch.float8_e4m3fn, out_scale=s)
+    two = torch.empty(2, *s.shape, dtype=torch.uint8, device="cuda").view(s.dtype)
+    two.view(torch.uint8)[0] = s.view(torch.uint8)
+    want = ops.matmul_fp8(q, s, b, bs, out_dtype=torch.float8_e4m3fn)
+    got = ops.matmul_fp8(q, two[0], b, bs, out_dtype=torch.float8_e4m3fn, out_scale=two[1])          # beside them
+    assert same(got, want) and torch.equal(two[0].view(torch.uint8), s.view(torch.uint8))
