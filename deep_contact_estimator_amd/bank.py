@@ -28,7 +28,8 @@ class contact_bank:
     """contact_cnn with a bank of FC heads.  precision: "bf16_fc" -- bf16 features, weights and activations, fp32 sums; "fp8_fc" -- fc.0 and
     fc.3 in e4m3 with a power of two for every 128 values (dce.h DCE_FP8_FC), the rest bf16.  max_batch, tune: contact_cnn's.
     Calls on CUDA tensors run on torch's current stream and may be captured once one has run; the conv stack's context serves one stream at a
-    time, replayed graphs included (as contact_cnn's)."""
+    time, replayed graphs included (as contact_cnn's).  load_state_dict ends the graphs captured before it: they hold the addresses of weights that
+    it gives back (as contact_cnn's do), so capture again."""
 
     def __init__(self, device=None, max_batch: int = 32768, precision: str = "bf16_fc", tune=None):
         if precision not in ("bf16_fc", "fp8_fc"):
@@ -37,10 +38,11 @@ class contact_bank:
         self._f8 = precision == "fp8_fc"
         self._heads: list[dict[str, np.ndarray]] = []
         self._layers = None
+        self._streams: set[int] = set()                    # that the layers' memory is known to be used on
 
     def load_state_dict(self, state_dict: Mapping, heads: Sequence[Mapping]):
         """state_dict: a checkpoint of the reference (its conv stack is used); heads: one mapping with the six fc.* keys for each head (a whole
-        checkpoint will do)."""
+        checkpoint will do).  Graphs captured before this call must not be replayed after it."""
         if not 1 <= len(heads) <= ops.GROUPS_MAX:
             raise RuntimeError(f"contact_bank: 1 .. {ops.GROUPS_MAX} heads, not {len(heads)}")
         shapes, found = dict(STATE_DICT_SHAPES), []
@@ -64,11 +66,16 @@ class contact_bank:
 
     def _on_device(self, device):
         """[(weights, scales, bias)] of the three layers, stacked over the heads."""
+        import torch
+        stream = torch.cuda.current_stream(device)
         if self._layers is not None and self._layers[0] == device:
+            if stream.cuda_stream not in self._streams:    # (memory of one stream's pool: given back, it is not to be used again before this stream is through with it)
+                for t in (t for layer in self._layers[1] for t in layer if t is not None):
+                    t.record_stream(stream)
+                self._streams.add(stream.cuda_stream)
             return self._layers[1]
         if not self._heads:
             raise RuntimeError("load_state_dict first: the bank has no heads")
-        import torch
         layers = []
         for key in ("fc.0", "fc.3", "fc.6"):
             shape = self._heads[0][key + ".weight"].shape
@@ -85,7 +92,8 @@ class contact_bank:
                     q, e = ops.quantize(v, rows=128)
                     w.view(torch.uint8)[i], s.view(torch.uint8)[i] = q.view(torch.uint8), e.view(torch.uint8)
             layers.append((w, s, torch.from_numpy(np.stack([h[key + ".bias"] for h in self._heads])).to(device)))
-        self._layers = (device, layers)
+        stream.synchronize()                               # (whatever stream the next call is on finds them whole)
+        self._layers, self._streams = (device, layers), {stream.cuda_stream}
         return layers
 
     def _run(self, x, head, raw_sequence: bool):
