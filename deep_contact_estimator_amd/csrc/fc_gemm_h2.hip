@@ -57,11 +57,14 @@ __device__ __forceinline__ unsigned h2_m0_begin(unsigned lds)
 // ("scc" in the clobber list is the fix of round 5's intermittent GPU memory fault: the s_add_u32 on m0 rewrites SCC, and without the clobber the scheduler
 //  was free to put this statement between the s_add_u32 and the s_addc_u32 that form the NEXT piece's 64-bit base -- the carry was lost, and a piece whose
 //  rows lie beyond a multiple of 4 GB that the operand buffer happens to cross was fetched from 4 GB below.  Seen in the assembly of all three K-split
-//  instantiations, the shipped fc.3 one among them; DESIGN.md 4.6, profiles/r6k_*.  -DH2_SCC_UNDECLARED=1: the old statement, for the A/B.)
+//  instantiations, the shipped fc.3 one among them; DESIGN.md 4.6, profiles/r6k_*.  -DH2_SCC_UNDECLARED=1: the old statement, in
+//  device assembly alone, for the scan that has to find it.)
 #ifndef H2_SCC_UNDECLARED
 #define H2_SCC_UNDECLARED 0
 #elif H2_SCC_UNDECLARED && !DCE_EXPERIMENTS
 #error "H2_SCC_UNDECLARED reproduces a bug: experiments builds only"
+#elif H2_SCC_UNDECLARED && !defined(__HIP_DEVICE_COMPILE__)
+#error "H2_SCC_UNDECLARED is there to be looked for in device assembly: no library that can be loaded is built with it"
 #endif
 __device__ __forceinline__ void h2_piece(const char* base, unsigned v)
 {

@@ -22,23 +22,19 @@ pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-def _stress(*args, expect_fault=False, timeout=900):
+def _stress(*args, timeout=900):
     r = subprocess.run([sys.executable, os.path.join(ROOT, "tools", "guard_stress.py"), *args], env=dict(os.environ, PYTHONPATH=ROOT),
                        capture_output=True, text=True, timeout=timeout, cwd=ROOT)
-    if expect_fault:
-        assert r.returncode != 0 and "Memory access fault" in (r.stdout + r.stderr), (r.returncode, (r.stdout + r.stderr)[-1500:])
-        return None
     assert r.returncode == 0, (r.returncode, (r.stdout + r.stderr)[-3000:])
     j = json.loads([l for l in r.stdout.splitlines() if l.startswith("{")][-1])
     assert j["ok"] and not j["mismatches"], j
     return j
 
 
-@pytest.mark.skip(reason="reads out of bounds on purpose: the GPU memory fault that it waits for takes the whole machine's GPU with it where faults are not contained "
-                         "(the process then reports 'an illegal memory access' instead of the runtime's own message)")
+@pytest.mark.skip(reason="read out of bounds on purpose: the GPU memory fault that it waited for takes the whole machine's GPU with it where faults are not contained")
 def test_guard_placement_catches_an_overrun_of_one_window():
-    """The instrument works: a caller that claims ONE window more than its guard-placed input buffer holds dies with a GPU memory fault."""
-    _stress("--precision", "fp32", "--cycles", "1", "--guard", "1", "--device-io", "--overrun", "1", "--sizes", "1281", "--sequence", "0", expect_fault=True)
+    """A caller that claims one window more than its guard-placed input buffer holds dies with a GPU memory fault.  Nothing provokes that any more
+    (tests/test_no_fault_on_purpose.py); what the placement found while it did is in profiles/r6l_scc_clobber_ab.txt."""
 
 
 @pytest.mark.parametrize("precision", ["fp32", "fp32_f16x2", "bf16_fc"])
@@ -56,20 +52,15 @@ def test_product_precisions_stay_inside_their_buffers(precision):
 @pytest.mark.parametrize("precision", ["fp32", "fp32_f16x2", "bf16_fc"])
 def test_product_precisions_with_a_4gb_line_inside_every_buffer(precision):
     """Placement 3: a multiple of 4 GB inside every buffer of the context and of the caller -- a 64-bit address whose carry was lost lands on an unmapped
-    page.  (The statement that lost it faults here in the first cycle: tools/guard_trace7.sh, profiles/r6l_scc_clobber_ab.txt.)"""
+    page.  (The statement that lost it faulted here in the first cycle: profiles/r6l_scc_clobber_ab.txt.)"""
     j = _stress("--precision", precision, "--cycles", "12", "--guard", "3", "--device-io")
     assert j["guard"] == 3 and j["cycles"] == 12
 
 
+@pytest.mark.skip(reason="ran a library that faults the GPU; tests/test_build.py finds the statement in the assembly, on the CPU")
 def test_the_undeclared_scc_statement_faults_under_placement_3():
-    """The A/B build with the OLD asm statement (libdce_h2sccbug.so, when it has been built: tools/guard_trace7.sh says how) dies in its first guarded
-    cycle on the PRODUCT plan of fp32_f16x2 -- the instrument sees the bug the fix removed."""
-    lib = os.path.join(ROOT, "deep_contact_estimator_amd", "libdce_h2sccbug.so")
-    if not os.path.exists(lib):
-        pytest.skip("libdce_h2sccbug.so not built (build.build_variant('h2sccbug', ['-DDCE_EXPERIMENTS=1', '-DH2_SCC_UNDECLARED=1']))")
-    r = subprocess.run([sys.executable, os.path.join(ROOT, "tools", "guard_stress.py"), "--precision", "fp32_f16x2", "--cycles", "2", "--guard", "3", "--device-io",
-                        "--sizes", "4100", "--sequence", "0"], env=dict(os.environ, PYTHONPATH=ROOT, DCE_LIB=lib), capture_output=True, text=True, timeout=600, cwd=ROOT)
-    assert r.returncode != 0 and "Memory access fault" in (r.stdout + r.stderr), (r.returncode, (r.stdout + r.stderr)[-1500:])
+    """The old asm statement in a library of its own dies in its first guarded cycle (profiles/r6l_scc_clobber_ab.txt).  Such a library can no longer be
+    built: the statement compiles to device assembly alone."""
 
 
 def test_latency_mode_stays_inside_its_buffers():
