@@ -1188,12 +1188,14 @@ long long row_tiles(const ProductArgs& p, int bm)                             //
     return p.offsets ? (long long)p.m / bm + (p.groups < p.m ? p.groups : p.m) : ((long long)p.m + bm - 1) / bm;
 }
 
+bool fits(long long workgroups, int threads) { return workgroups * threads < 1ll << 32; }      // (a launch has fewer than 2^32 threads)
+
 template <int IN, int OUT, class T>
 hipError_t launch_any(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long grid = (row_tiles(p, T::BM) * p.tiles_n + 7) / 8 * 8;
-    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    if (!fits(grid, T::THREADS)) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> devices{0};
     const hipError_t e = allow_lds(reinterpret_cast<const void*>(product_any_kernel<IN, OUT, T>), T::LDS, devices);
     if (e != hipSuccess) return e;
@@ -1206,7 +1208,7 @@ hipError_t launch_ring(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
-    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    if (!fits(grid, T::THREADS)) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> devices{0};
     const hipError_t e = allow_lds(reinterpret_cast<const void*>(product_ring_kernel<IN, OUT, T>), T::LDS, devices);
     if (e != hipSuccess) return e;
@@ -1219,7 +1221,7 @@ hipError_t launch_phased(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
-    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    if (!fits(grid, T::THREADS)) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> devices{0};
     const hipError_t e = allow_lds(reinterpret_cast<const void*>(product_phased_kernel<IN, OUT, T>), T::LDS, devices);
     if (e != hipSuccess) return e;
@@ -1232,7 +1234,7 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + 15) / 16;
     const long long grid = (row_tiles(p, MT * 16) * p.tiles_n + 7) / 8 * 8;
-    if (grid > 0x7fffffffll) return hipErrorInvalidConfiguration;
+    if (!fits(grid, 1024)) return hipErrorInvalidConfiguration;
     product_rows_kernel<IN, OUT, MT, U><<<(unsigned)grid, 1024, 0, st>>>(p);
     return hipGetLastError();
 }
@@ -1270,7 +1272,7 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     int best = -1;
     double least = 0;
     auto offer = [&](int kernel, bool can, int bm, int bn, double edge, double step) {
-        if (!can) return;
+        if (!can || !fits((row_tiles(p, bm) * ((p.n + bn - 1) / bn) + 7) / 8 * 8, bn == 16 ? 1024 : 512)) return;
         const double rows = p.groups > 1 ? (double)p.m / bm + 0.5 * (p.groups < p.m ? p.groups : p.m) : (double)((p.m + bm - 1) / bm);   // (a group's last tile is half full)
         const double us = 2 + ceil(rows * ((p.n + bn - 1) / bn) / 256) * (edge + steps * step);
         if (best < 0 || us < least) { best = kernel; least = us; }
@@ -1285,6 +1287,7 @@ hipError_t launch_out(const ProductArgs& p, hipStream_t st)
     offer(P128, dma, 128, 256, 4, F == 0 ? 1.03 : F == 1 ? 1.13 : 1.75);
     offer(P192, dma && F < 2, 192, 256, 4, F == 0 ? 1.30 : 1.44);             // (16-bit operands do not fit its registers)
     offer(P256, dma && (F == 0 || (F == 1 && p.kbytes % KROW == 0)), 256, 256, 5, F == 0 ? 1.60 : 1.90);
+    if (best < 0) return hipErrorInvalidConfiguration;
     if constexpr (OUT != OUT_E4M3) {
         if (best == ROWS16) return launch_rows<IN, OUT, 1, 3>(p, st);
         if (best == ROWS32) return launch_rows<IN, OUT, 2, 2>(p, st);

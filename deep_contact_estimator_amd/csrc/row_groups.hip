@@ -159,28 +159,29 @@ __global__ __launch_bounds__(256) void decide_kernel(const float* __restrict__ l
                                                      float* __restrict__ out, int* __restrict__ pred, unsigned char* __restrict__ contacts)
 {
     const int c = threadIdx.x & 15;
-    const long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (i >= n) return;
-    const long long s = index ? (long long)index[i] : i;
-    const float v = s >= 0 && s < rows ? logits[s * 16 + c] : __builtin_nanf("");
-    if (out) out[i * 16 + c] = v;
-    float best = v; int at = c;
+    for (long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i < n; i += (long long)gridDim.x * 16) {
+        const long long s = index ? (long long)index[i] : i;
+        const float v = s >= 0 && s < rows ? logits[s * 16 + c] : __builtin_nanf("");
+        if (out) out[i * 16 + c] = v;
+        float best = v; int at = c;
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-        const float o = __shfl_xor(best, d); const int oc = __shfl_xor(at, d);
-        const bool on = o != o, bn = best != best;
-        const bool take = on ? (!bn || oc < at) : (!bn && (o > best || (o == best && oc < at)));
-        if (take) { best = o; at = oc; }
-    }
-    if (c == 0) {
-        if (pred) pred[i] = at;
-        if (contacts) for (int b = 0; b < 4; ++b) contacts[i * 4 + b] = (unsigned char)((at >> (3 - b)) & 1);
+        for (int d = 1; d < 16; d <<= 1) {
+            const float o = __shfl_xor(best, d); const int oc = __shfl_xor(at, d);
+            const bool on = o != o, bn = best != best;
+            const bool take = on ? (!bn || oc < at) : (!bn && (o > best || (o == best && oc < at)));
+            if (take) { best = o; at = oc; }
+        }
+        if (c == 0) {
+            if (pred) pred[i] = at;
+            if (contacts) for (int b = 0; b < 4; ++b) contacts[i * 4 + b] = (unsigned char)((at >> (3 - b)) & 1);
+        }
     }
 }
 
 hipError_t launch_decide(const float* logits, long long n, long long rows, const int* index, float* out, int* pred, unsigned char* contacts, hipStream_t st)
 {
-    decide_kernel<<<(unsigned)((n + 15) / 16), 256, 0, st>>>(logits, n, rows, index, out, pred, contacts);
+    const long long wgs = (n + 15) / 16, most = 1 << 20;                      // (a launch has fewer than 2^32 threads; up to 16 million rows each workgroup takes its sixteen)
+    decide_kernel<<<(unsigned)(wgs < most ? wgs : most), 256, 0, st>>>(logits, n, rows, index, out, pred, contacts);
     return hipGetLastError();
 }
 

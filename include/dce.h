@@ -381,7 +381,8 @@ int  dce_quantize(int device_id, void* hip_stream, const dce_quantize_desc* d);
  * or e4m3, a product of a group of eight loses less than 2^-13 of the group's largest besides: a sum is off by up to 7 * 2^-13 of the sum of its products'
  * magnitudes (1.5e-5 of a result on random operands, 7e-5 where all have one sign, and any part of one that cancels).  y is rounded once to y_type; e4m3
  * results take dce_quantize's power of two for every 128 columns of a row, y_scale[(c / 128) * ld_y_scale + j], in scale_type: that of the exact sums where
- * products and bias have one sign (values near a border are summed again in fp32), otherwise that of sums off by no more than the above.  Any m, n and k (k = 0: the bias); strides in values; 16-byte
+ * products and bias have one sign (values near a border are summed again in fp32), otherwise that of sums off by no more than the above.  Any m, n and k (k = 0: the bias; refused beyond
+ * 2^23 tiles, 128 x 128 of a result from rows at any address and 256 x 256 from aligned ones); strides in values; 16-byte
  * aligned rows run fastest.  y and y_scale overlap nothing that the
  * call reads, nor each other (refused where they are found to: rows of different strides that interleave are not looked into).  The same call gives the same bits. */
 typedef struct dce_matmul_desc {
