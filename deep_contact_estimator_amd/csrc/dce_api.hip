@@ -1081,6 +1081,7 @@ int dce_finalize_weights(dce_ctx* c, int precision)
 #endif
     DEVICE_GUARD(c);
     { const int rc = lat_quiesce(c); if (rc) return rc; }
+    c->finalized = false;                                  // (until the end: what fails on the way leaves weights of two precisions, or none)
     // a captured online graph holds the old weight pointers / precision: drop it, the next push re-captures
     if (c->online_exec) { hipGraphExecDestroy(c->online_exec); c->online_exec = nullptr; }
     if (c->online_graph) { hipGraphDestroy(c->online_graph); c->online_graph = nullptr; }
