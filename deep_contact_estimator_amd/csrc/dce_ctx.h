@@ -142,6 +142,7 @@ inline int fail(dce_ctx* c, int code, const char* fmt, ...)
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     if (c) c->err = buf; else dce::g_create_error = buf;
+    if (code == DCE_ERR_HIP) (void)hipGetLastError();      // (it is reported here: the next launch asks the runtime for its last error, and would report it again)
     return code;
 }
 

@@ -35,11 +35,26 @@ rc = lib.dce_finalize_weights(ctx, 4)
 assert rc == -2, (rc, lib.dce_last_error(ctx))
 rc, said, _ = run()
 assert rc == -3 and b"not finalized" in said, (rc, said)
+MORE
 lib.dce_destroy(ctx)
 print("fine")
 """
+AGAIN = CODE.replace("MORE\n", """
+_lib.check(lib.dce_finalize_weights(ctx, 1), ctx)
+rc, said, again = run()
+assert rc == 0 and np.array_equal(want, again), (rc, said)
+""")
+
+
+def ends_well(code):
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=ROOT, DCE_GUARD_ALIGN=str(1 << 60)), capture_output=True, text=True, timeout=100, cwd=ROOT)
+    assert r.returncode == 0 and "fine" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-1500:])
 
 
 def test_a_failed_finalize_leaves_no_context_that_runs():
-    r = subprocess.run([sys.executable, "-c", CODE], env=dict(os.environ, PYTHONPATH=ROOT, DCE_GUARD_ALIGN=str(1 << 60)), capture_output=True, text=True, timeout=100, cwd=ROOT)
-    assert r.returncode == 0 and "fine" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-1500:])
+    ends_well(CODE.replace("MORE\n", ""))
+
+
+def test_a_failure_is_reported_once():
+    """finalized again, the context serves: the runtime's last error is not taken for one of the launches'"""
+    ends_well(AGAIN)
