@@ -43,6 +43,7 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, Place& a
     int total = 0;
     if (!p.offsets) total = (p.m + bm - 1) / bm;
     else for (int base = 0; base < p.groups; base += 64) total += scan(base);
+    if ((unsigned)total > (unsigned)p.tiles_m) total = p.tiles_m;             // (offsets that fall: tiles of the same rows, of which the launch has no more than these)
     const unsigned all = (unsigned)total * (unsigned)p.tiles_n, per = (all + 7) >> 3, slot = blockIdx.x >> 3, id = (blockIdx.x & 7) * per + slot;
     if (slot >= per || id >= all) return false;
     const unsigned band = id / ((unsigned)total * 8), wide = p.tiles_n - band * 8 < 8 ? p.tiles_n - band * 8 : 8, in = id - band * total * 8;
@@ -57,7 +58,7 @@ __device__ __forceinline__ bool find_tile(const ProductArgs& p, int bm, Place& a
             at.g = base + w;
             at.first = __builtin_amdgcn_readlane(lo, w) + (t - (before + __builtin_amdgcn_readlane(sum, w) - __builtin_amdgcn_readlane(tiles, w))) * bm;
             at.end = __builtin_amdgcn_readlane(hi, w);
-            return true;
+            return at.first >= __builtin_amdgcn_readlane(lo, w) && at.first < at.end;       // (... and their count may pass 32 bits)
         }
         before += here;
     }
@@ -1194,6 +1195,7 @@ template <int IN, int OUT, class T>
 hipError_t launch_any(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
+    p.tiles_m = (int)row_tiles(p, T::BM);
     const long long grid = (row_tiles(p, T::BM) * p.tiles_n + 7) / 8 * 8;
     if (!fits(grid, T::THREADS)) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> devices{0};
@@ -1207,6 +1209,7 @@ template <int IN, int OUT, class T>
 hipError_t launch_ring(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
+    p.tiles_m = (int)row_tiles(p, T::BM);
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
     if (!fits(grid, T::THREADS)) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> devices{0};
@@ -1220,6 +1223,7 @@ template <int IN, int OUT, class T>
 hipError_t launch_phased(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + T::BN - 1) / T::BN;
+    p.tiles_m = (int)row_tiles(p, T::BM);
     const long long tiles = row_tiles(p, T::BM) * p.tiles_n, grid = (tiles + 7) / 8 * 8;
     if (!fits(grid, T::THREADS)) return hipErrorInvalidConfiguration;
     static std::atomic<unsigned long long> devices{0};
@@ -1233,6 +1237,7 @@ template <int IN, int OUT, int MT, int U>
 hipError_t launch_rows(ProductArgs p, hipStream_t st)
 {
     p.tiles_n = (p.n + 15) / 16;
+    p.tiles_m = (int)row_tiles(p, MT * 16);
     const long long grid = (row_tiles(p, MT * 16) * p.tiles_n + 7) / 8 * 8;
     if (!fits(grid, 1024)) return hipErrorInvalidConfiguration;
     product_rows_kernel<IN, OUT, MT, U><<<(unsigned)grid, 1024, 0, st>>>(p);

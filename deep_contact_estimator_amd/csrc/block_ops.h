@@ -25,7 +25,7 @@ struct ProductArgs {
     const int* offsets; const int* index;
     long long a_rows;                         // rows of a: an index outside reads as a row of zeros
     int m, n, kbytes, groups, relu;
-    int tiles_n;
+    int tiles_n, tiles_m;                     // column tiles; row tiles, at most
 };
 
 struct QuantArgs {

@@ -39,3 +39,20 @@ def test_a_product_of_as_many_rows_as_there_may_be(m, k):
     want = a.float().sum(1).bfloat16()
     for lo in range(0, m, 1 << 26):
         assert torch.equal(y[lo:lo + (1 << 26), 0], want[index[lo:lo + (1 << 26)].long()])
+
+
+def test_offsets_that_fall_again_and_again():
+    """0, m, 0, m, ..: 512 groups of all m rows each, more tiles than 32 bits count.  The launch is as large as m rows need: what it computes is right and
+    what it does not is left alone, and nothing is written beside the result"""
+    m, groups, k = 1 << 28, 1024, 16
+    a = torch.arange(2 * k, device="cuda").view(2, k).bfloat16()
+    w = torch.ones(groups, 1, k, dtype=torch.bfloat16, device="cuda")
+    offsets = (torch.arange(groups + 1, device="cuda") % 2 * m).int()
+    index = torch.arange(m, dtype=torch.int32, device="cuda").remainder_(2)
+    big = torch.full((m + 512, 1), 9.0, dtype=torch.bfloat16, device="cuda")
+    ops.matmul_grouped(a, w, offsets, index=index, out=big[256:256 + m])
+    want = a.float().sum(1).bfloat16()
+    assert (big[:256] == 9).all() and (big[256 + m:] == 9).all()
+    for lo in range(0, m, 1 << 26):
+        y = big[256 + lo:256 + lo + (1 << 26), 0]
+        assert ((y == want[index[lo:lo + (1 << 26)].long()]) | (y == 9)).all()
