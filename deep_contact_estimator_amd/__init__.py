@@ -7,10 +7,10 @@ built library; using the model does (there is no CPU fallback).
 from .contact_cnn import contact_cnn, load_checkpoint          # noqa: F401
 from . import synth                                              # noqa: F401
 
-__all__ = ["contact_cnn", "contact_bank", "load_checkpoint", "ops", "synth"]
+__all__ = ["contact_cnn", "load_checkpoint", "synth"]              # (without contact_bank and ops, which import torch: `import *` works where there is none)
 
 
-def __getattr__(name):                                             # (these import torch: only when asked for)
+def __getattr__(name):                                             # (only when asked for)
     import importlib
     if name == "ops":
         return importlib.import_module(".ops", __name__)
