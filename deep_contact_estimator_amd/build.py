@@ -53,30 +53,50 @@ def built_hash(lib: str = LIB) -> str | None:
 ENTRIES, ENTRIES_SOURCE = os.path.join(HERE, "_entries.so"), "torch_entries.cpp"
 
 
+def entries_abi() -> str:
+    """What _entries.so is made for: a torch and an interpreter."""
+    import sysconfig
+    import torch
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _entries_command() -> list[str]:
+    import sysconfig
+    import torch
+    t = os.path.dirname(torch.__file__)
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DDCE_ENTRIES_ABI="{entries_abi()}"',
+            "-isystem", os.path.join(t, "include"), "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, ENTRIES_SOURCE), "-o", ENTRIES + ".tmp",
+            "-L", os.path.join(t, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+
+
+def entries_hash() -> str:
+    """sha256 over what _entries.so is compiled from: the source, the header it takes, and the command with the torch and the interpreter in it."""
+    import hashlib
+    h = hashlib.sha256("\0".join(_entries_command()).replace(HERE, "").encode())
+    for path in (os.path.join(CSRC, ENTRIES_SOURCE), os.path.join(HERE, "..", "include", "dce.h")):
+        h.update(open(path, "rb").read())
+    return h.hexdigest()
+
+
 def build_entries(force: bool = False) -> str | None:
     """_entries.so: ops.py's entries on torch tensors (csrc/torch_entries.cpp), a CPython extension module compiled against the installed torch; None
     without torch (the package works on numpy arrays without it)."""
     try:
-        import torch
+        import torch                                              # noqa: F401
     except ImportError:
         return None
-    import hashlib
-    import sysconfig
-    h = hashlib.sha256(torch.__version__.encode())
-    for path in (os.path.join(CSRC, ENTRIES_SOURCE), os.path.join(HERE, "..", "include", "dce.h")):
-        h.update(open(path, "rb").read())
-    if not force and os.path.exists(ENTRIES) and built_hash(ENTRIES) == h.hexdigest():
+    if not force and os.path.exists(ENTRIES) and built_hash(ENTRIES) == entries_hash():
         return ENTRIES
-    t = os.path.dirname(torch.__file__)
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-isystem", os.path.join(t, "include"), "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, ENTRIES_SOURCE), "-o", ENTRIES + ".tmp",
-           "-L", os.path.join(t, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    cmd = _entries_command()
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"no host compiler for {ENTRIES_SOURCE}: {e}") from e
     if r.returncode != 0:
         raise RuntimeError("compile failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
     os.replace(ENTRIES + ".tmp", ENTRIES)
     with open(ENTRIES + ".srchash", "w") as f:
-        f.write(h.hexdigest() + "\n")
+        f.write(entries_hash() + "\n")
     return ENTRIES
 
 

@@ -318,4 +318,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_entries", "ops.py's entries on to
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__entries() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__entries()
+{
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "ABI", DCE_ENTRIES_ABI) != 0) { Py_DECREF(m); return nullptr; }       // (the torch and the interpreter it was compiled for: build.py)
+    return m;
+}

@@ -35,6 +35,9 @@ def _entries():
         from . import _entries as e
     except ImportError as err:
         raise RuntimeError(f"{_lib.ENTRIES_PATH} does not load ({err}): build it with `python -m deep_contact_estimator_amd.build`") from err
+    from .build import entries_abi
+    if getattr(e, "ABI", None) != entries_abi():
+        raise RuntimeError(f"{_lib.ENTRIES_PATH} was built for {getattr(e, 'ABI', 'another torch')}, this is {entries_abi()}: build it with `python -m deep_contact_estimator_amd.build`")
     address = lambda f: C.cast(f, C.c_void_p).value                # noqa: E731
     e.bind(*(address(f) for f in (lib.dce_quantize, lib.dce_matmul, lib.dce_group_rows, lib.dce_group_rows_work, lib.dce_decide, lib.dce_last_error)),
            torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (lambda device: 0), _lib.DceError)
