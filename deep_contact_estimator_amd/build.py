@@ -143,12 +143,25 @@ def build_variant(name: str, defines: list[str], force: bool = True) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """libdce.so, then _entries.so, which only ops.py needs: where that one does not compile (torch without a host compiler or Python's headers) the library
+    is there all the same, a warning says why, and ops.py that it is missing."""
+    lib = _build_lib(force, verbose)
+    try:
+        build_entries(force)
+    except RuntimeError as e:
+        import warnings
+        if os.path.exists(ENTRIES) and built_hash(ENTRIES) != entries_hash():
+            os.remove(ENTRIES)                                    # (of other sources)
+        warnings.warn(f"{ENTRIES} was not built: {e}")
+    return lib
+
+
+def _build_lib(force: bool, verbose: bool) -> str:
     """hipcc -c each translation unit for gfx950, then link WITHOUT naming a HIP runtime:
     libdce.so leaves hip* undefined so that it binds to the ONE runtime already in the process
     (PyTorch wheels bundle their own libamdhip64/libhsa-runtime64; a second copy from
     /opt/rocm in the same process cannot open the device).  _lib.load() puts the right runtime
     in the global symbol scope first."""
-    build_entries(force)
     if not force and not stale():
         return LIB
     os.makedirs(OBJDIR, exist_ok=True)

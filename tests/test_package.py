@@ -41,3 +41,23 @@ def test_the_extension_module_belongs_to_one_torch_and_one_interpreter(monkeypat
         m.setattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", not torch._C._GLIBCXX_USE_CXX11_ABI)
         assert build.entries_hash() != here
     assert build.entries_hash() == here
+
+
+@pytest.mark.parametrize("compiler", ["/nonexistent/g++", "false"])
+def test_the_library_is_built_where_the_extension_module_is_not(monkeypatch, tmp_path, compiler):
+    pytest.importorskip("torch")
+    from deep_contact_estimator_amd import build
+    made = []
+    monkeypatch.setattr(build, "_build_lib", lambda force, verbose: made.append(force) or "libdce.so")
+    monkeypatch.setattr(build, "ENTRIES", str(tmp_path / "_entries.so"))
+    command = build._entries_command()
+    monkeypatch.setattr(build, "_entries_command", lambda: [compiler, *command[1:]])
+    with pytest.warns(UserWarning, match="_entries.so was not built"):
+        assert build.build() == "libdce.so"
+    assert made == [False]
+    (tmp_path / "_entries.so").write_bytes(b"of other sources")
+    with pytest.warns(UserWarning, match="_entries.so was not built"):
+        build.build()
+    assert not (tmp_path / "_entries.so").exists()
+    with pytest.raises(RuntimeError):
+        build.build_entries()
