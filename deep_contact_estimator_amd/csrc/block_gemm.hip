@@ -563,7 +563,8 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, f32x4 (&acc)[T:
 #pragma unroll 4
                 for (int t = 0; t < T::NT * 4; ++t) {
                     const int row = (t * 64 + lane) / (T::NT * 16), c = (t * 64 + lane) % (T::NT * 16);
-                    const E v = *reinterpret_cast<const E*>(turn + row * PITCH + c * SZ);
+                    E v;
+                    __builtin_memcpy(&v, turn + row * PITCH + c * SZ, SZ);    // (written as words: to the compiler another type's memory)
                     if (j0 + row < end && n0 + wn + c < p.n) *reinterpret_cast<E*>(y0 + (long long)(j0 + row) * p.y_row + c * SZ) = v;
                 }
             }
