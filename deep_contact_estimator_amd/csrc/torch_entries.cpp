@@ -232,6 +232,8 @@ PyObject* matmul(PyObject* const* arg)
     d.out_type = (int32_t)out_type;
     d.relu = relu;
     check(f_matmul(dev, stream_of(dev), &d));
+    for (PyObject* o : {arg[8], arg[9]})                            // a caller's tensors were written in place: autograd has to know, as of torch's own operators
+        if (o != Py_None && !THPVariable_Unpack(o).is_inference()) THPVariable_Unpack(o).unsafeGetTensorImpl()->bump_version();
     return out_type == DCE_TYPE_E4M3 ? pair(std::move(out), std::move(outs)) : THPVariable_Wrap(std::move(out));
 }
 

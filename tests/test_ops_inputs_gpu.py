@@ -75,3 +75,26 @@ def test_results_on_the_scales_that_a_product_reads_are_refused():
     want = ops.matmul_fp8(q, s, b, bs, out_dtype=torch.float8_e4m3fn)
     got = ops.matmul_fp8(q, two[0], b, bs, out_dtype=torch.float8_e4m3fn, out_scale=two[1])          # beside them
     assert same(got, want) and torch.equal(two[0].view(torch.uint8), s.view(torch.uint8))
+
+
+def test_writing_to_out_is_told_to_autograd():
+    """a tensor that a backward pass still needs, given as `out` meanwhile: the backward pass refuses it, as after torch's own in-place operators"""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, w = torch.randn(8, 16, generator=g, device="cuda"), torch.randn(1, 16, 16, generator=g, device="cuda").bfloat16()
+    offsets = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    out = torch.ones(8, 16, device="cuda")
+    p = torch.ones(8, 16, device="cuda", requires_grad=True)
+    y = (p * out).sum()
+    before = out._version
+    ops.matmul_grouped(x.bfloat16(), w, offsets, out_dtype=torch.float32, out=out)
+    assert out._version == before + 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    (q, s), (b, bs) = ops.quantize(torch.randn(8, 256, generator=g, device="cuda")), ops.quantize(torch.randn(130, 256, generator=g, device="cuda"), rows=128)
+    out, scale = torch.empty(8, 130, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(2, 8, dtype=torch.uint8, device="cuda").view(s.dtype)
+    versions = out._version, scale._version
+    ops.matmul_fp8(q, s, b, bs, out_dtype=out.dtype, out=out, out_scale=scale)
+    assert (out._version, scale._version) == (versions[0] + 1, versions[1] + 1)
+    with torch.inference_mode():
+        out = torch.empty(8, 16, device="cuda")
+    ops.matmul_grouped(x.bfloat16(), w, offsets, out_dtype=torch.float32, out=out)                 # (has no version)
