@@ -55,7 +55,7 @@ SYMBOLS = {
     "dce_debug_alloc": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p)]),
     "dce_debug_free": (C.c_int, [C.c_void_p, C.c_void_p]),
     "dce_features": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p]),
-    "dce_quantize": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),                    # descriptors are packed with struct (ops.py)
+    "dce_quantize": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),                    # descriptors: csrc/torch_entries.cpp fills them; from Python, bytes of the struct
     "dce_matmul": (C.c_int, [C.c_int, C.c_void_p, C.c_char_p]),
     "dce_group_rows_work": (C.c_int64, [C.c_int64, C.c_int]),
     "dce_group_rows": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),

@@ -142,8 +142,9 @@ __device__ __forceinline__ void spoil(f32x4 (&acc)[NT], unsigned bad)
 // acc += the product of a block of 16 x 16 over one step of K.
 //
 // The 8-bit matrix instruction lines the eight products of a group up with the largest of them and keeps 13 bits below its leading one (measured: of
-// 65536 + 8 everything, of 65536 + 4 nothing is left of the second; between groups sums are fp32): on random operands 1.5e-5 of the result, a hundredth
-// of the rounding to bf16 (1.7e-3) and less still of that to e4m3, so results in those types take it.  fp32 results would be a hundred times worse
+// 65536 + 8 everything, of 65536 + 4 nothing is left of the second, -4 neither; between groups sums are fp32): on random operands 1.5e-5 of the result, with
+// products of one sign 7e-5, at worst 7 * 2^-13 of the sum of magnitudes.  The rounding to bf16 is 1.7e-3 of a result and that to e4m3 more, so results in
+// those types take it (and e4m3 scales look again next to their borders).  fp32 results would be a hundred times worse
 // than their type: their operands go through the 16-bit instructions, at half the rate, whose sums of 32 products are good to 1e-8 -- with e8m0 scales
 // as bf16 with the scale in it, with fp32 scales as fp16 (every e4m3 number is one).
 //
@@ -901,7 +902,9 @@ __global__ __launch_bounds__(T::THREADS, 2) void product_any_kernel(ProductArgs 
 //
 // What bounds it, at 8192 x 2048 over long K: 1.10 us a step of 256 x 256 (zeros: the clock at its highest), with or without its requests, 0.87 of them
 // matrix instructions and the rest the phases' barriers; 1.39 with random operands, where the power limit sets the clock (a library product of one scale
-// for all: 0.86 and 1.18).  Requests between matrix instructions took 1.45 and 1.7 there.  8192^3: e4m3 2680 TFLOP/s, bf16 1390.
+// for all: 0.86 and 1.18).  Requests between matrix instructions took 1.45 and 1.7 there.  Counters, 32768 rows of 2048 x 4736: 546 thousand cycles with
+// zeros and with random operands, 238 and 264 .. 284 us; the matrix pipe is busy in 56 % of them, a wave waits in 38 % of its own; 4 % of the LDS cycles are
+// conflicts, 78 % of the requests find their line in the L2.  8192^3: e4m3 415 us, 2650 TFLOP/s; bf16 781, 1408.
 template <int WM_, int WN_, int MT_, int NT_, int NBUF_> struct Phased {
     static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, NBUF = NBUF_;
     static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, WAVES = WM * WN, THREADS = 64 * WAVES;
@@ -1249,21 +1252,21 @@ hipError_t launch_rows(ProductArgs p, hipStream_t st)
 // fitted to runs on 1 .. 32768 rows of 2048 x 4736 and 512 x 2048 and to grouped ones (a graph of 20 calls each; us):
 //
 //   rows   e4m3 to bf16:   16 / 32 at a time   32 x 128   64 x 128   128 x 128   128 x 256   192 x 256   256 x 256
-//        1                       5.5 /  6.2       14.3       16.6
-//       32                       7.3 /  9.5       14.5       16.8
-//      128                      25.8 / 18.5       15.6       17.3
-//     1024                                        30.3       19.8        26.2        32.5        47.7        53.6
-//     2048                                        55.3       36.5        31.2        34.9        49.4        55.2
-//     4096                                                               57.1        46.2        52.9        57.5
-//     5000                                                               75.2        67.8        55.2        58.4
-//     8192                                                              104.5        78.6        95.7        71.9
-//    32768                                       941.9      626.2       383.1       303.2       300.4       259.6
+//        1                       5.8 /  6.4       14.1       16.5
+//       32                       7.5 /  9.4       14.4       16.8
+//      128                      23.3 / 17.7       15.2       17.0
+//     1024                                        29.6       19.3        24.8        30.6        47.6        54.4
+//     2048                                        55.1       35.1        26.6        31.1        48.1        55.0
+//     4096                                                               53.1        39.2        50.4        56.5
+//     5000                                                               72.5        63.6        51.5        56.6
+//     8192                                                               98.5        76.0        99.8        65.3
+//    32768                                       833        527         387         297         299         257
 //
-// Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 11.0 | 17.2, 3000 23.7 | 19.3, 20000 118 | 93; 4096 167 | 99.
+// Operands at any address (1001 x 1419; 2048 x 4729), 32 x 128 tiles | 128 x 128:  733 rows 10.6 | 16.8, 3000 31.3 | 18.3, 20000 189 | 92; 4096 212 | 98.
 //
-// Folded block sums (fp32 scales) take 1.02 .. 1.2 times as long (32768 rows 305), 16-bit operands from e4m3 (fp32 results) 1.35 times in the rings and
-// 1.4 .. 1.9 in the large tiles (2048 rows 43.3, 32768 499 with e8m0 scales and 542 with fp32 ones), bf16 operands over the same K twice, since a step of
-// K is 64 of theirs (4096 rows 78.7 in 128 x 256 tiles, 32768 478 in 256 x 256).  A K that ends inside a step costs up to 5 %.
+// Folded block sums (fp32 scales) take 1.02 .. 1.2 times as long (32768 rows 311), 16-bit operands from e4m3 (fp32 results) 1.35 times in the rings and
+// 1.4 .. 2 in the large tiles (2048 rows 48.7, 32768 527 with e8m0 scales and 569 with fp32 ones), bf16 operands over the same K twice, since a step of
+// K is 64 of theirs (4096 rows 74.8 in 128 x 256 tiles, 32768 484 in 256 x 256).  A K that ends inside a step costs up to 5 %.
 template <int IN, int OUT>
 hipError_t launch_out(const ProductArgs& p, hipStream_t st)
 {

@@ -4,7 +4,8 @@
 //
 // A power of two costs a floating-point format nothing: x * 2^-e is exact, so q carries the ONE rounding to 4 significant bits, and the matrix pipe
 // can apply the exponents itself.  NaN and infinities become NaN and do not set the scale.
-// Bound: memory, one read of x and one write of q: 32768 x 4736 bf16 83 us, 5.6 TB/s; one row 2.5 us, the launch.
+// Bound: memory, one read of x and one write of q: 32768 x 4736 bf16 83 us, 5.6 TB/s; one row 2.5 us, the launch; weights, 2048 x 4736
+// fp32, 10.4 us, 4.7 TB/s (592 workgroups, each one block: a read, a barrier and a write).
 #include "block_ops.h"
 
 namespace dce {

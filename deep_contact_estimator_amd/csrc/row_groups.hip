@@ -154,7 +154,7 @@ hipError_t launch_group_rows(const void* ids, int id_bytes, int n, int groups, i
 }
 
 // ---- logits -> class and contact bits, the row of logits picked by `index` (first of equal ones; a NaN is the largest, the first NaN wins; an index
-//      outside the rows: NaN logits, class 0).  Sixteen lanes a row.
+//      outside the rows: NaN logits, class 0).  Sixteen lanes a row.  4096 rows 2.8 us; 200000 in another order (28 MB) 15.3.
 __global__ __launch_bounds__(256) void decide_kernel(const float* __restrict__ logits, long long n, long long rows, const int* __restrict__ index,
                                                      float* __restrict__ out, int* __restrict__ pred, unsigned char* __restrict__ contacts)
 {

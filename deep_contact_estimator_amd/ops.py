@@ -64,8 +64,8 @@ def _out(what, dtype):
 
 def matmul_fp8(a, a_scale, b, b_scale, bias=None, relu: bool = False, out_dtype=torch.bfloat16, out=None, out_scale=None):
     """act(a @ b.T + bias) of e4m3 operands: a (m, k) with a_scale (ceil(k / 128), m), b (n, k) with b_scale (ceil(n / 128),
-    ceil(k / 128)), as quantize makes them or of any value (float32); bias (n,) float32; act = ReLU if relu.  Sums are fp32 and
-    are rounded once to out_dtype: float32, bfloat16, or float8_e4m3fn -- then (q, scale) with a power of two for every 128 columns of a
+    ceil(k / 128)), as quantize makes them, or float32 numbers of which the products of one of a and one of b are normal float32
+    numbers or zero; bias (n,) float32; act = ReLU if relu.  Sums are fp32 and are rounded once to out_dtype: float32, bfloat16, or float8_e4m3fn -- then (q, scale) with a power of two for every 128 columns of a
     row, in the operands' scale dtype: the next product's a and a_scale.  For bfloat16 and float8_e4m3fn results the matrix instruction
     drops less than 2^-13 of the largest of eight products from each of the others: sums are off by up to 7 * 2^-13 of the sum of
     their products' magnitudes, 1.5e-5 of a result on random operands; where products cancel, more of it, and an e4m3 scale may
