@@ -100,7 +100,7 @@ class contact_bank:
         import torch
         if not _is_torch(head):
             head = torch.from_numpy(np.ascontiguousarray(head))
-        if head.dtype.is_floating_point or head.dtype.is_complex:
+        if head.numel() and (head.dtype.is_floating_point or head.dtype.is_complex):             # (an empty list has no type of its own)
             raise RuntimeError(f"contact_bank: head must be whole numbers, got {head.dtype}")     # (-0.5 is no head: rounded towards zero it would be one)
         host = not (_is_torch(x) and x.is_cuda)
         if host:

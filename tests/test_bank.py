@@ -14,3 +14,14 @@ def test_heads_are_whole_numbers(head):
             bank.predict(x, head)
     with pytest.raises(RuntimeError, match="whole numbers"):
         bank.infer_sequence(np.zeros((151, 54), np.float32), head)
+
+
+def test_no_windows_and_no_heads():
+    """an empty list, which numpy takes for floats, is no wrong type: the call ends where a call without a device ends"""
+    from deep_contact_estimator_amd import _lib, contact_bank, synth
+    if _lib.load().dce_device_count() > 0:
+        pytest.skip("GPU present")
+    bank = contact_bank(max_batch=4).load_state_dict(synth.make_state_dict(1), [synth.make_state_dict(1)])
+    for head in ([], np.zeros(0), torch.zeros(0)):
+        with pytest.raises(RuntimeError, match="no HIP device|no CPU"):
+            bank.predict(np.zeros((0, 150, 54), np.float32), head)

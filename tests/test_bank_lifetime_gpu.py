@@ -48,3 +48,13 @@ def test_the_first_call_on_another_stream_finds_the_weights_whole():
     assert all(torch.equal(o, bank.predict(x, head)["logits"]) for o in out)
     assert len(bank._streams) == 4
     bank._conv.close()
+
+
+def test_no_windows():
+    sd = synth.make_state_dict(1, "uniform")
+    bank = contact_bank(device=0, max_batch=8).load_state_dict(sd, [sd])
+    for x in (torch.zeros(0, 150, 54), torch.zeros(0, 150, 54, device="cuda")):
+        for head in ([], torch.zeros(0), torch.zeros(0, dtype=torch.int32, device="cuda")):
+            out = bank.predict(x, head)
+            assert out["logits"].shape == (0, 16) and out["pred"].shape == (0,) and out["contacts"].shape == (0, 4)
+    bank._conv.close()
