@@ -53,7 +53,7 @@ class contact_bank:
             one = {}
             for k in HEAD_KEYS:
                 v = h[k].detach().cpu().numpy() if _is_torch(h[k]) else h[k]
-                one[k] = np.ascontiguousarray(np.asarray(v), dtype=np.float32)
+                one[k] = np.array(v, dtype=np.float32, order="C")         # (a copy: what the caller does to its arrays later is not the bank's)
                 if one[k].shape != shapes[k]:
                     raise RuntimeError(f"contact_bank: head {i}: size mismatch for {k}: {one[k].shape}, model {shapes[k]}")
             found.append(one)

@@ -111,7 +111,7 @@ class contact_cnn:
             v = state_dict[k]
             if _is_torch(v):
                 v = v.detach().cpu().numpy()
-            a = np.ascontiguousarray(np.asarray(v), dtype=np.float32)
+            a = np.array(v, dtype=np.float32, order="C")                  # (a copy, as torch's own load_state_dict makes: the weights go up with the first call)
             if a.shape != shape:
                 raise RuntimeError(f"size mismatch for {k}: checkpoint {a.shape}, model {shape}")
             self._state[k] = a

@@ -25,3 +25,21 @@ def test_no_windows_and_no_heads():
     for head in ([], np.zeros(0), torch.zeros(0)):
         with pytest.raises(RuntimeError, match="no HIP device|no CPU"):
             bank.predict(np.zeros((0, 150, 54), np.float32), head)
+
+
+@pytest.mark.parametrize("kind", ["numpy", "torch"])
+def test_loaded_weights_are_the_callers_no_longer(kind):
+    """arrays that change after load_state_dict (a training loop's parameters) change neither the model nor the bank, whose weights go up with the first call"""
+    from deep_contact_estimator_amd import contact_bank, contact_cnn, synth
+    sd = {k: np.array(v) for k, v in synth.make_state_dict(1).items()}
+    want = {k: v.copy() for k, v in sd.items()}
+    given = {k: torch.from_numpy(v) for k, v in sd.items()} if kind == "torch" else sd
+    model = contact_cnn(max_batch=4)
+    model.load_state_dict(given)
+    bank = contact_bank(max_batch=4).load_state_dict(given, [given, given])
+    for v in sd.values():
+        v += 1
+    for held in (model.state_dict(), bank._conv.state_dict()):
+        assert all(np.array_equal(held[k], want[k]) for k in want)
+    for head in bank._heads:
+        assert head and all(np.array_equal(head[k], want[k]) for k in head)
