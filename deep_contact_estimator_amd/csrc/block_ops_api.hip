@@ -37,7 +37,9 @@ bool apart(const Rows& r, int64_t count, int64_t step, const Rows& w)
 {
     if (step == 0) count = 1;
     if (r.rows < 1 || r.width < 1 || w.rows < 1 || w.width < 1 || w.end() <= r.at || r.end() + (uintptr_t)((count - 1) * step) <= w.at) return true;
-    for (int64_t g = 0; g < count; ++g) { Rows m = r; m.at += (uintptr_t)(g * step); if (!apart(m, w)) return false; }
+    const int64_t first = r.end() > w.at || count == 1 ? 0 : (int64_t)((w.at - r.end()) / step) + 1;          // (the matrices that reach w at all)
+    const int64_t behind = count == 1 ? 1 : (int64_t)((w.end() - 1 - r.at) / step) + 1;
+    for (int64_t g = first; g < count && g < behind; ++g) { Rows m = r; m.at += (uintptr_t)(g * step); if (!apart(m, w)) return false; }
     return true;
 }
 // one run of n values

@@ -140,3 +140,16 @@ def test_decide(lib, no_gpu):   # noqa: F811
                 assert call(**{one: at[other] + size[other]})[0] == -2
     assert call(out=at["logits"], index=0)[0] == -2                   # in place, row for row
     assert call(out=at["logits"] + 64, index=0)[0] == -1
+
+
+def test_many_matrices_are_looked_through_quickly(lib, no_gpu):   # noqa: F811
+    """65535 matrices of x and as many of q between them: no pair of them all is compared with every other"""
+    import time
+    d = dict(x=1 << 30, ldx=64, x_batch=4096, q=(1 << 30) + 4096, ldq=64, q_batch=16384, scale=1 << 40, batch=65535, rows=16, k=64, block_rows=128, x_type=0, scale_type=0)
+    at = time.monotonic()
+    assert accepted(lib, lib.dce_quantize, _quantize(**d))
+    assert answer(lib, lib.dce_quantize, _quantize(**{**d, "q": d["q"] - 1}))[0] == -1           # the last byte of every matrix of x
+    last = {**d, "q": d["x"] + 65534 * 16384 + 4095}                    # ... of the last one alone
+    assert answer(lib, lib.dce_quantize, _quantize(**last))[0] == -1
+    assert accepted(lib, lib.dce_quantize, _quantize(**{**last, "q": last["q"] + 1}))
+    assert time.monotonic() - at < 2
